@@ -53,7 +53,9 @@ def _needs_build(src: str, obj: str) -> bool:
     if not os.path.exists(obj):
         return True
     omt = os.path.getmtime(obj)
-    deps = [src] + [os.path.join(CSRC, h) for h in ("common.h", "mfma_tile.h")]
+    # this file holds the compiler's flags
+    deps = [src, os.path.abspath(__file__)] + [
+        os.path.join(CSRC, h) for h in ("common.h", "mfma_tile.h")]
     return any(os.path.getmtime(d) > omt for d in deps if os.path.exists(d))
 
 
@@ -75,9 +77,12 @@ def build(verbose: bool = False) -> None:
         obj = os.path.join(OBJ, f.replace(".hip", ".o"))
         objs.append(obj)
         if _needs_build(src, obj):
+            # no packed fp32 arithmetic: the compiler forms it from plain
+            # float code, and it has given wrong results on this hardware
             jobs.append([f"{ROCM}/bin/hipcc", "--offload-arch=gfx950", "-O3",
-                         "-std=c++17", "-fPIC", *defs, *incs, "-c", src,
-                         "-o", obj])
+                         "-std=c++17", "-fPIC", "-Xclang",
+                         "-target-feature", "-Xclang", "-packed-fp32-ops",
+                         *defs, *incs, "-c", src, "-o", obj])
     for f in CPP_SOURCES:
         src = os.path.join(CSRC, f)
         obj = os.path.join(OBJ, f.replace(".cpp", ".o"))

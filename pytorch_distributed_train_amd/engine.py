@@ -22,7 +22,7 @@ from .ops import functional as OF
 from .parallel.comm import make_communicator, NullComm
 from .parallel.ddp import GradReducer
 from .parallel.flat import FlatParams
-from .parallel.optim import FusedSGD
+from .parallel.optim import FusedAdamW, FusedSGD
 from .parallel.sync_bn import convert_sync_batchnorm
 from .utils.amp import GradScaler
 from .utils.watchdog import Watchdog
@@ -92,9 +92,19 @@ class Trainer:
         if self.device.type == "cuda" \
                 and not os.environ.get("PDTA_NO_DIRECT_GRAD"):
             self._wire_direct_grads()
-        self.optimizer = FusedSGD(self.flat, lr=args.lr,
-                                  momentum=args.momentum,
-                                  weight_decay=args.weight_decay)
+        if getattr(args, "optimizer", "sgd") == "adamw":
+            decay = ((lambda name, shape: len(shape) > 1)
+                     if args.no_decay_1d else None)
+            self.optimizer = FusedAdamW(self.flat, lr=args.lr,
+                                        betas=tuple(args.adam_betas),
+                                        eps=args.adam_eps,
+                                        weight_decay=args.weight_decay,
+                                        state_bits=args.adam_bits,
+                                        decay=decay, seed=args.seed)
+        else:
+            self.optimizer = FusedSGD(self.flat, lr=args.lr,
+                                      momentum=args.momentum,
+                                      weight_decay=args.weight_decay)
         self.scaler = GradScaler(enabled=(args.amp and args.dtype == "fp16"))
         self.packs = None
         if self.device.type == "cuda" and self.compute_dtype != torch.float32:

@@ -38,6 +38,16 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--warmup-epochs", type=int, default=0)
     p.add_argument("--momentum", type=float, default=0.9)
     p.add_argument("--weight-decay", type=float, default=1e-4)
+    p.add_argument("--optimizer", default="sgd", choices=("sgd", "adamw"))
+    p.add_argument("--adam-betas", type=float, nargs=2,
+                   default=(0.9, 0.999), metavar=("BETA1", "BETA2"))
+    p.add_argument("--adam-eps", type=float, default=1e-8)
+    p.add_argument("--adam-bits", type=int, default=32, choices=(8, 32),
+                   help="AdamW states: fp32, or 8 bits with a scale per 64 "
+                        "elements")
+    p.add_argument("--no-decay-1d", action="store_true",
+                   help="AdamW: no weight decay on biases and norms "
+                        "(parameters of one dimension)")
     p.add_argument("--dtype", default="bf16", choices=("fp32", "bf16", "fp16"),
                    help="compute dtype for activations/GEMMs; master weights fp32")
     p.add_argument("--sync-bn", action="store_true",

@@ -101,6 +101,8 @@ void pdta_attn_fused_bwd_ds(const void*, const void*, const void*, void*,
                             hipStream_t);
 }
 
+void bind_transformer(pybind11::module_& m);  // bind_transformer.cpp
+
 namespace {
 
 int dt_of(const at::Tensor& t) {
@@ -1060,4 +1062,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rccl_allgather", &rccl_allgather);
   m.def("rccl_comm_destroy", &rccl_comm_destroy);
   m.def("rccl_comm_abort", &rccl_comm_abort);
+  bind_transformer(m);
 }

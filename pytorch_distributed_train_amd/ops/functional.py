@@ -891,3 +891,134 @@ class AttentionQKVFn(torch.autograd.Function):
 
 def attention_qkv(qkv2d, b, s, h, hd, nvalid, scale):
     return AttentionQKVFn.apply(qkv2d, b, s, h, hd, nvalid, scale)
+
+
+# ---------------------------------------------------------------------------
+# AdamW over flat storage
+# ---------------------------------------------------------------------------
+
+ADAMW_BLOCK = 64          # elements under one 8-bit scale, one decay byte
+_ADAMW_TINY = 2.0 ** -100  # a block whose largest is below is stored as 0
+
+
+def _scale8(x):
+    top = x.abs().view(-1, ADAMW_BLOCK).amax(1)
+    dead = top < _ADAMW_TINY
+    scale = (top * (1.0 / 448.0)).masked_fill(dead, 0.0)
+    inv = (top.reciprocal() * 448.0).masked_fill(dead, 0.0)
+    return scale, inv.repeat_interleave(ADAMW_BLOCK)
+
+
+def adamw_quantize(x, positive: bool = False):
+    """fp32 [n] -> (float8_e4m3fn [n], fp32 scale [n/64]), to the nearest;
+    x is about value * scale of its block of 64. positive (x >= 0): what is
+    above 0 stays above 0, as sqrt(v) has to."""
+    scale, inv = _scale8(x)
+    y = (x * inv).clamp(-448.0, 448.0)
+    if positive:
+        y = torch.where(y > 0, y.clamp(min=2.0 ** -9), y)
+    return y.to(torch.float8_e4m3fn), scale
+
+
+def adamw_dequantize(codes, scale):
+    """Inverse of adamw_quantize, in fp32."""
+    return codes.float() * scale.repeat_interleave(ADAMW_BLOCK)
+
+
+def _adamw_noise(n, step, seed, device):
+    # 16 random bits an element: the halves of a mix of its pair's index,
+    # the step and the seed, as in csrc/adamw.hip
+    low = 0xFFFFFFFF
+    x = torch.arange(n // 2, dtype=torch.int64, device=device)
+    x = (x * 0x9E3779B1 + step * 0x6A09E667 + seed * 0x3B67AE85) & low
+    x = ((x ^ (x >> 16)) * 0x3C6EF373) & low
+    x = ((x ^ (x >> 15)) * 0x254FF53B) & low
+    x = x ^ (x >> 16)
+    return torch.stack([x & 0xFFFF, x >> 16], 1).view(-1).float()
+
+
+def _adamw_quantize_random(x, step, seed):
+    scale, inv = _scale8(x)
+    y = (x * inv).clamp(max=448.0)
+    # the distance of neighbouring e4m3 values: 2^(exponent - 3)
+    unit = torch.ldexp(torch.ones_like(y),
+                       torch.frexp(y.clamp(min=2.0 ** -6))[1] - 4)
+    r = _adamw_noise(x.numel(), step, seed, x.device) * 2.0 ** -16
+    z = (torch.floor(y / unit + r) * unit).clamp(max=448.0)
+    z = torch.where(y > 0, z.clamp(min=2.0 ** -9), y)
+    return z.to(torch.float8_e4m3fn), scale
+
+
+@torch.no_grad()
+def adamw_step(p, g, m, v, step, lr, beta1=0.9, beta2=0.999, eps=1e-8,
+               weight_decay=0.01, decay=None, grad_scale=1.0, m_scale=None,
+               v_scale=None, seed=0):
+    """One AdamW step in place over flat fp32 storage p with gradient g
+    (torch.optim.AdamW's formula; n a multiple of 64):
+
+        step += 1;  g = g * grad_scale
+        m = beta1 m + (1-beta1) g;   v = beta2 v + (1-beta2) g^2
+        p = p (1 - lr weight_decay decay)
+              - lr/(1-beta1^step) m / (sqrt(v)/sqrt(1-beta2^step) + eps)
+
+    step: one int64 on p's device, advanced here, so a captured step replays
+    as the next one. lr: a number, or one float32 on p's device.
+    decay: None, or uint8 [n/64], 0 where weight decay is left out.
+    States: m, v fp32; or, with m_scale and v_scale (fp32 [n/64]),
+    float8_e4m3fn of m and of sqrt(v) over a scale per 64 elements, sqrt(v)
+    rounded up or down at random by a mix of element, step and seed. A
+    gradient that is not finite makes p's element NaN and its block's 8-bit
+    state not finite. GPU: csrc/adamw.hip, two launches."""
+    if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
+        raise ValueError(f"betas must be in [0, 1): {beta1}, {beta2}")
+    if eps < 0.0:
+        raise ValueError(f"eps must not be negative: {eps}")
+    n = p.numel()
+    if n % ADAMW_BLOCK:
+        raise ValueError(f"p must have a multiple of {ADAMW_BLOCK} elements, "
+                         f"has {n}")
+    if (m_scale is None) != (v_scale is None):
+        raise ValueError("m_scale and v_scale come together")
+    lr_dev = lr if isinstance(lr, torch.Tensor) else None
+    if p.is_cuda:
+        ext().adamw_step(p, g, m, v, step,
+                         0.0 if lr_dev is not None else float(lr), lr_dev,
+                         beta1, beta2, eps, weight_decay, decay, grad_scale,
+                         m_scale, v_scale, seed & 0xFFFFFFFF)
+        return
+    state = torch.float32 if m_scale is None else torch.float8_e4m3fn
+    for name, t, dtype, size in (
+            ("p", p, torch.float32, n), ("g", g, torch.float32, n),
+            ("m", m, state, n), ("v", v, state, n),
+            ("m_scale", m_scale, torch.float32, n // ADAMW_BLOCK),
+            ("v_scale", v_scale, torch.float32, n // ADAMW_BLOCK),
+            ("decay", decay, torch.uint8, n // ADAMW_BLOCK),
+            ("step", step, torch.int64, 1)):
+        if t is not None and (t.dtype != dtype or t.numel() != size
+                              or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous {dtype} with "
+                             f"{size} elements")
+    step += 1
+    t = int(step)
+    if lr_dev is not None:
+        lr = float(lr_dev)
+    if m_scale is None:
+        m32, v32 = m, v
+    else:
+        m32 = adamw_dequantize(m, m_scale)
+        v32 = adamw_dequantize(v, v_scale).square_()
+    gs = g if grad_scale == 1.0 else g * grad_scale
+    m32.mul_(beta1).add_(gs * (1.0 - beta1))
+    v32.mul_(beta2).add_(gs * gs * (1.0 - beta2))
+    on = 1.0 if decay is None \
+        else decay.repeat_interleave(ADAMW_BLOCK).float()
+    p.mul_(1.0 - lr * weight_decay * on)
+    bc1, bc2 = 1.0 - beta1 ** t, 1.0 - beta2 ** t
+    p.sub_((lr / bc1) * m32 / (v32.sqrt() / bc2 ** 0.5 + eps))
+    if m_scale is not None:
+        for (codes, scale), (c, s) in (
+                (adamw_quantize(m32), (m, m_scale)),
+                (_adamw_quantize_random(v32.sqrt(), t, seed & 0xFFFFFFFF),
+                 (v, v_scale))):
+            c.copy_(codes)
+            s.copy_(scale)

@@ -1,7 +1,8 @@
 from .flat import FlatParams
 from .comm import make_communicator, NullComm, TorchDistComm
 from .ddp import GradReducer, DistributedDataParallel
-from .optim import FusedSGD
+from .optim import FusedAdamW, FusedSGD
 
 __all__ = ["FlatParams", "make_communicator", "NullComm", "TorchDistComm",
-           "GradReducer", "DistributedDataParallel", "FusedSGD"]
+           "GradReducer", "DistributedDataParallel", "FusedAdamW",
+           "FusedSGD"]

@@ -1,4 +1,5 @@
-// Python binding of the transformer-training operators (AdamW).
+// Python binding of the transformer-training operators (AdamW,
+// query/key norm with rotation).
 // Arguments are checked here, before a launch: a kernel's bounds rest on them.
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
@@ -6,10 +7,18 @@
 
 #include <hip/hip_runtime_api.h>
 
+#include <vector>
+
 extern "C" {
 void pdta_adamw(float*, const float*, void*, void*, float*, float*, long,
                 long*, float, const float*, double, double, float, float,
                 const unsigned char*, float, unsigned, void*, hipStream_t);
+int pdta_qknorm_rows(long, int, int);
+void pdta_qknorm(const void* const*, const long*, const void* const*,
+                 const long*, const float* const*, void* const*, const int*,
+                 const float*, const float*, const void*, int, int, int, int,
+                 long, long, float, int, int, int, float*, float*, float*,
+                 int, hipStream_t);
 }
 
 namespace {
@@ -37,6 +46,15 @@ void check_flat(const char* name, const at::Tensor& t, const at::Tensor& like,
               " must be contiguous with ", numel, " elements");
   TORCH_CHECK((uintptr_t)t.data_ptr() % 16 == 0, name,
               " must start at a multiple of 16 bytes");
+}
+
+int dt_of(const at::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return 0;
+    case at::kBFloat16: return 1;
+    case at::kHalf: return 2;
+    default: TORCH_CHECK(false, "unsupported dtype ", t.scalar_type());
+  }
 }
 
 void adamw_step(at::Tensor p, at::Tensor g, at::Tensor m, at::Tensor v,
@@ -83,6 +101,141 @@ void adamw_step(at::Tensor p, at::Tensor g, at::Tensor m, at::Tensor v,
   launched("adamw_step");
 }
 
+// ---- query/key norm and rotation -----------------------------------------
+// q [b, s, h, hd], k [b, s, hk, hd]; a dimension of one element has no
+// stride to speak of
+bool rows8(const at::Tensor& t) {
+  if ((uintptr_t)t.data_ptr() % 16) return false;
+  for (int d = 0; d < 3; ++d)
+    if (t.size(d) > 1 && t.stride(d) % 8) return false;
+  return true;
+}
+
+// dq, dk undefined: forward -> {q', k'}; else backward -> {dx_q, dx_k,
+// dw_q, dw_k} (the last two empty without weights)
+std::vector<at::Tensor> qk_norm_rope(
+    at::Tensor q, at::Tensor k, c10::optional<at::Tensor> wq,
+    c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cos,
+    c10::optional<at::Tensor> sin, c10::optional<at::Tensor> positions,
+    double eps, bool interleaved, c10::optional<at::Tensor> dq,
+    c10::optional<at::Tensor> dk) {
+  TORCH_CHECK(q.is_cuda(), "q must be on GPU");
+  c10::DeviceGuard guard(q.device());
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) &&
+                  q.size(1) == k.size(1) && q.size(3) == k.size(3),
+              "q and k must be [b, s, heads, hd], alike but for the heads");
+  long b = q.size(0), s = q.size(1), hd = q.size(3);
+  TORCH_CHECK(hd >= 1 && hd <= 256, "head size must be 1 to 256, is ", hd);
+  TORCH_CHECK(b * s < (1l << 31) && q.size(2) + k.size(2) < 65536,
+              "too many rows");
+  bool bwd = dq.has_value();
+  TORCH_CHECK(bwd == dk.has_value(), "dq and dk come together");
+  bool norm = wq.has_value();
+  TORCH_CHECK(norm == wk.has_value(), "q_weight and k_weight come together");
+  at::Tensor t[2] = {q, k}, d[2];
+  if (bwd) d[0] = *dq, d[1] = *dk;
+  bool vec = hd % 8 == 0;
+  const void *x[2], *dy[2] = {nullptr, nullptr};
+  long xs[6], gs[6] = {0, 0, 0, 0, 0, 0};
+  const float* w[2] = {nullptr, nullptr};
+  int heads[2];
+  for (int i = 0; i < 2; ++i) {
+    TORCH_CHECK(t[i].device() == q.device() &&
+                    t[i].scalar_type() == q.scalar_type(),
+                "q and k must have one device and dtype");
+    TORCH_CHECK(hd == 1 || t[i].numel() == 0 || t[i].stride(3) == 1,
+                "heads must be contiguous in memory");
+    vec = vec && rows8(t[i]);
+    x[i] = t[i].data_ptr();
+    heads[i] = t[i].size(2);
+    for (int j = 0; j < 3; ++j) xs[3 * i + j] = t[i].stride(j);
+    if (bwd) {
+      TORCH_CHECK(d[i].device() == q.device() &&
+                      d[i].scalar_type() == q.scalar_type() &&
+                      d[i].sizes() == t[i].sizes() &&
+                      (hd == 1 || d[i].numel() == 0 || d[i].stride(3) == 1),
+                  "a gradient must be like its output");
+      vec = vec && rows8(d[i]);
+      dy[i] = d[i].data_ptr();
+      for (int j = 0; j < 3; ++j) gs[3 * i + j] = d[i].stride(j);
+    }
+    if (norm) {
+      const at::Tensor& wt = i ? *wk : *wq;
+      TORCH_CHECK(wt.device() == q.device() &&
+                      wt.scalar_type() == at::kFloat && wt.numel() == hd &&
+                      wt.is_contiguous(),
+                  "weights must be contiguous float32 [", hd, "] on ",
+                  q.device());
+      vec = vec && (uintptr_t)wt.data_ptr() % 16 == 0;
+      w[i] = wt.data_ptr<float>();
+    }
+  }
+  long rot = 0, npos = 0;
+  bool pos32 = false;
+  TORCH_CHECK(cos.has_value() == sin.has_value(),
+              "cos and sin come together");
+  TORCH_CHECK(cos.has_value() || norm, "neither weights nor tables");
+  if (cos.has_value()) {
+    TORCH_CHECK(cos->dim() == 2 && cos->sizes() == sin->sizes() &&
+                    cos->device() == q.device() &&
+                    sin->device() == q.device() &&
+                    cos->scalar_type() == at::kFloat &&
+                    sin->scalar_type() == at::kFloat &&
+                    cos->is_contiguous() && sin->is_contiguous(),
+                "cos and sin must be contiguous float32 [positions, rot/2] "
+                "on ",
+                q.device());
+    npos = cos->size(0);
+    rot = 2 * cos->size(1);
+    TORCH_CHECK(rot >= 2 && rot <= hd, "tables for ", rot,
+                " elements, heads have ", hd);
+    TORCH_CHECK(npos < (1l << 31), "too many positions");
+    TORCH_CHECK(positions.has_value() || s <= npos, "tables for ", npos,
+                " positions, sequences of ", s);
+    vec = vec && rot % (interleaved ? 8 : 16) == 0 &&
+          (uintptr_t)cos->data_ptr() % 16 == 0 &&
+          (uintptr_t)sin->data_ptr() % 16 == 0;
+  }
+  if (positions.has_value()) {
+    TORCH_CHECK(positions->device() == q.device() &&
+                    positions->is_contiguous() &&
+                    positions->numel() == b * s,
+                "positions must be contiguous [b, s] on ", q.device());
+    pos32 = positions->scalar_type() == at::kInt;
+    TORCH_CHECK(pos32 || positions->scalar_type() == at::kLong,
+                "positions must be int32 or int64");
+  }
+  at::Tensor y[2];
+  void* yp[2];
+  for (int i = 0; i < 2; ++i) {
+    y[i] = at::empty({b, s, heads[i], hd}, q.options());
+    yp[i] = y[i].data_ptr();
+  }
+  at::Tensor part, dwq, dwk;
+  auto f32 = q.options().dtype(at::kFloat);
+  if (bwd && norm) {
+    int rows = pdta_qknorm_rows(b * s, heads[0] + heads[1], vec);
+    if (rows == 0)
+      return {y[0], y[1], at::zeros({hd}, f32), at::zeros({hd}, f32)};
+    part = at::empty({rows, 2 * hd}, f32);
+    dwq = at::empty({hd}, f32);
+    dwk = at::empty({hd}, f32);
+  }
+  pdta_qknorm(x, xs, dy, gs, w, yp, heads,
+              rot ? cos->data_ptr<float>() : nullptr,
+              rot ? sin->data_ptr<float>() : nullptr,
+              positions.has_value() ? positions->data_ptr() : nullptr, pos32,
+              npos, rot, hd, b, s, (float)eps, interleaved, vec, bwd,
+              bwd && norm ? part.data_ptr<float>() : nullptr,
+              bwd && norm ? dwq.data_ptr<float>() : nullptr,
+              bwd && norm ? dwk.data_ptr<float>() : nullptr, dt_of(q),
+              cur_stream());
+  launched("qk_norm_rope");
+  if (!bwd) return {y[0], y[1]};
+  if (!norm) return {y[0], y[1], at::Tensor(), at::Tensor()};
+  return {y[0], y[1], dwq, dwk};
+}
+
 }  // namespace
 
 void bind_transformer(pybind11::module_& m) {
@@ -91,4 +244,9 @@ void bind_transformer(pybind11::module_& m) {
         py::arg("beta1"), py::arg("beta2"), py::arg("eps"),
         py::arg("weight_decay"), py::arg("decay"), py::arg("grad_scale"),
         py::arg("m_scale"), py::arg("v_scale"), py::arg("seed"));
+  m.def("qk_norm_rope", &qk_norm_rope, py::arg("q"), py::arg("k"),
+        py::arg("q_weight"), py::arg("k_weight"), py::arg("cos"),
+        py::arg("sin"), py::arg("positions"), py::arg("eps"),
+        py::arg("interleaved"), py::arg("dq") = py::none(),
+        py::arg("dk") = py::none());
 }

@@ -894,6 +894,174 @@ def attention_qkv(qkv2d, b, s, h, hd, nvalid, scale):
 
 
 # ---------------------------------------------------------------------------
+# Query/key norm with the position rotation
+# ---------------------------------------------------------------------------
+
+def rope_tables(n: int, rot_dim: int, theta: float = 10000.0,
+                scale: float = 1.0, device=None):
+    """(cos, sin), fp32 [n, rot_dim/2], of the angles
+    position / scale * theta^(-2i/rot_dim). scale > 1 squeezes longer
+    sequences into the positions a model has seen. Angles are formed in 64
+    bits: in 32 those of far positions are off by more than 1e-3."""
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rot_dim must be even and positive: {rot_dim}")
+    f = theta ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64,
+                                device=device) / rot_dim)
+    a = torch.arange(n, dtype=torch.float64, device=device) / scale
+    a = a[:, None] * f
+    return a.cos().float(), a.sin().float()
+
+
+def _wide(x):
+    # the CPU reference computes in fp32; fp64 stays, for differences
+    return x if x.dtype == torch.float64 else x.float()
+
+
+def _rotate(x, cos, sin, interleaved):
+    """x [b, s, h, hd] with its first 2*cos.shape[-1] elements turned;
+    cos, sin [b or 1, s, 1, rot/2]."""
+    half = cos.shape[-1]
+    rot = 2 * half
+    if interleaved:
+        a, b = x[..., 0:rot:2], x[..., 1:rot:2]
+        y = torch.stack([a * cos - b * sin, b * cos + a * sin], -1).flatten(-2)
+    else:
+        a, b = x[..., :half], x[..., half:rot]
+        y = torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
+    return torch.cat([y, x[..., rot:]], -1)
+
+
+def _gathered(cos, sin, positions, s):
+    """Rows of the tables for every token; a position outside them turns by
+    NaN, as in the kernel."""
+    if positions is None:
+        return cos[:s][None, :, None], sin[:s][None, :, None]
+    ok = (positions >= 0) & (positions < cos.shape[0])
+    at = positions.long().clamp(0, cos.shape[0] - 1)
+    bad = (~ok)[:, :, None]
+    return tuple(t[at].masked_fill(bad, float("nan"))[:, :, None]
+                 for t in (cos, sin))
+
+
+def _inner1(x):
+    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+
+
+class QKNormRopeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, cos, sin, positions, eps, interleaved,
+                gslot_q, gslot_k):
+        ctx.eps, ctx.interleaved = eps, interleaved
+        ctx.gslot = (gslot_q, gslot_k)
+        ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
+        if q.is_cuda:
+            return tuple(ext().qk_norm_rope(
+                _inner1(q), _inner1(k), wq, wk, cos, sin, positions, eps,
+                interleaved))
+
+        def one(x, w):
+            x32 = _wide(x)
+            if w is not None:
+                r = (x32.square().mean(-1, keepdim=True) + eps).rsqrt()
+                x32 = x32 * r * _wide(w)
+            if cos is not None:
+                c, s = _gathered(cos, sin, positions, x.shape[1])
+                x32 = _rotate(x32, c, s, interleaved)
+            return x32.to(x.dtype)
+
+        return one(q, wq), one(k, wk)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
+        if q.is_cuda:
+            dq, dk, dwq, dwk = ext().qk_norm_rope(
+                _inner1(q), _inner1(k), wq, wk, cos, sin, positions, ctx.eps,
+                ctx.interleaved, dq=_inner1(dq), dk=_inner1(dk))
+        else:
+            def one(x, w, dy):
+                g = _wide(dy)
+                if cos is not None:
+                    c, s = _gathered(cos, sin, positions, x.shape[1])
+                    g = _rotate(g, c, -s, ctx.interleaved)
+                if w is None:
+                    return g.to(x.dtype), None
+                x32 = _wide(x)
+                r = (x32.square().mean(-1, keepdim=True) + ctx.eps).rsqrt()
+                xhat = x32 * r
+                dw = (g * xhat).sum((0, 1, 2))
+                g = g * _wide(w)
+                dx = r * (g - xhat * (g * xhat).mean(-1, keepdim=True))
+                return dx.to(x.dtype), dw
+
+            dq, dwq = one(q, wq, dq)
+            dk, dwk = one(k, wk, dk)
+        dw = [dwq, dwk]
+        for i, slot in enumerate(ctx.gslot):
+            if slot is not None and dw[i] is not None:
+                slot[0].copy_(dw[i])
+                if slot[1] is not None:
+                    slot[1]()
+                dw[i] = None
+        return (dq, dk, *dw, None, None, None, None, None, None, None)
+
+
+def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None,
+                 positions=None, eps: float = 1e-6, interleaved: bool = False,
+                 gslot_q=None, gslot_k=None):
+    """RMS norm of every query and key head with the position rotation in
+    the same pass: (q', k'), contiguous.
+
+    q [b, s, h, hd], k [b, s, hk, hd]: bf16, fp16 or fp32, any strides (the
+    views of one projection's output need no copy), hd up to 256.
+    q_weight, k_weight: fp32 [hd], both or neither (no norm).
+    cos, sin: fp32 [positions, rot/2] (rope_tables), both or neither (no
+    rotation); rot <= hd, the rest of the head is left as it is. Pairs are
+    (i, i + rot/2), or (2i, 2i+1) when interleaved.
+    positions: int32 or int64 [b, s], None for 0..s-1. One outside the
+    tables turns by NaN. The tables have no gradient.
+    GPU: csrc/qknorm.hip, one launch (two in backward); 16-byte accesses
+    where hd % 8 == 0, rot % 16 == 0 (8 interleaved) and rows are aligned."""
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] \
+            or q.shape[3] != k.shape[3]:
+        raise ValueError("q and k must be [b, s, heads, hd], alike but for "
+                         f"the heads: {tuple(q.shape)}, {tuple(k.shape)}")
+    if q.dtype != k.dtype or q.device != k.device:
+        raise ValueError("q and k must have one dtype and device")
+    b, s, hd = q.shape[0], q.shape[1], q.shape[3]
+    if not 1 <= hd <= 256:
+        raise ValueError(f"head size must be 1 to 256: {hd}")
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("q_weight and k_weight come together")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together")
+    if q_weight is None and cos is None:
+        raise ValueError("neither weights nor tables: nothing to do")
+    for w in (q_weight, k_weight):
+        if w is not None and w.shape != (hd,):
+            raise ValueError(f"weights must be [{hd}]: {tuple(w.shape)}")
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape != sin.shape \
+                or not 2 <= 2 * cos.shape[1] <= hd:
+            raise ValueError("cos and sin must be [positions, rot/2] with "
+                             f"rot <= {hd}: {tuple(cos.shape)}, "
+                             f"{tuple(sin.shape)}")
+        if cos.requires_grad or sin.requires_grad:
+            raise ValueError("cos and sin have no gradient")
+        if positions is None and s > cos.shape[0]:
+            raise ValueError(f"tables for {cos.shape[0]} positions, "
+                             f"sequences of {s}")
+    if positions is not None and (
+            positions.shape != (b, s)
+            or positions.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"positions must be int32 or int64 [{b}, {s}]")
+    if positions is not None:
+        positions = positions.contiguous()
+    return QKNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions,
+                              eps, interleaved, gslot_q, gslot_k)
+
+
+# ---------------------------------------------------------------------------
 # AdamW over flat storage
 # ---------------------------------------------------------------------------
 

@@ -23,7 +23,7 @@ TORCH_DIR = os.path.dirname(os.path.abspath(torch.__file__))
 
 HIP_SOURCES = ["elementwise.hip", "bn.hip", "pool.hip", "sgd.hip", "ce.hip",
                "gemm.hip", "conv.hip", "ln.hip", "packs.hip", "gemm_strided.hip", "attn.hip",
-               "adamw.hip", "qknorm.hip"]
+               "adamw.hip", "qknorm.hip", "attn_recompute.hip"]
 CPP_SOURCES = ["bind.cpp", "bind_transformer.cpp"]
 
 SO_NAME = "_hip_ops" + sysconfig.get_config_var("EXT_SUFFIX")

@@ -1,0 +1,660 @@
+// Attention whose backward recomputes the probabilities: nothing of size
+// sq x sk is ever written.
+//
+//   S = scale Q K^T;  P = exp(S - lse);  O = P V
+//   D = rowsum(dO * O);  dV = P^T dO;  dP = dO V^T;  dS = P * (dP - D)
+//   dQ = scale dS K;  dK = scale dS^T Q
+// Query i of a sequence sees key j if i < q_len, j < kv_len and, when causal,
+// j <= i + kv_len - q_len (the last query sees the last key). A row that sees
+// no key gives 0 and takes no gradient (its lse is +inf, so P is 0).
+//
+// Heads: the g = h / hk query heads of one key head are g rows a position,
+// row r = position * g + head. Every kernel works on those packed rows, so a
+// key head's tiles serve all of its query heads and dK, dV sum over them in
+// registers, in a fixed order.
+//
+// Layout: 32x32x16 MFMA. Each wave keeps 32 rows (or keys) on the lanes: the
+// product that makes S is taken with the kept side as the B operand, so a
+// lane holds one row's scores in its accumulators, 16 of every 32 keys, and
+// the other half sits 32 lanes away. Row maxima and sums are then loops over
+// a lane's registers. Packed to 16 bits, the same registers ARE the B operand
+// of the next product (its k index runs over the keys in the order that the
+// accumulators hold them, and the A operand is fetched from LDS in that
+// order): P and dS never pass through LDS. The other operands stream through
+// LDS tiles of 64 rows, two buffers deep, filled by global-to-LDS loads;
+// lanes outside a sequence or past the head's end fetch zeros, so nothing
+// behind a sequence is ever read.
+//
+// LDS rows are 128 or 256 bytes; 16-byte chunk c of row r lies at
+// c ^ perm(r), perm(r) = r's bits (1,0,2): 8 neighbouring rows spread over
+// all banks both for row fragments (16 bytes of one row a lane) and for the
+// transposing reads, whose 4 rows x 32 bytes need different chunk pairs.
+#include "common.h"
+
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int TILE = 64;  // streamed rows a step
+
+template <typename T> struct Op;
+template <> struct Op<__hip_bfloat16> {
+  static DEV_INLINE f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+        __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+        0);
+  }
+  static DEV_INLINE unsigned pack(float a, float b) {
+    f32x2 f = {a, b};
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f, bf16x2));
+  }
+};
+template <> struct Op<__half> {
+  static DEV_INLINE f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(
+        __builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+        0);
+  }
+  static DEV_INLINE unsigned pack(float a, float b) {
+    f32x2 f = {a, b};
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f, f16x2));
+  }
+};
+
+struct View {  // [b, s, heads, hd] of a 16-bit type, strides in elements
+  const void* p;
+  long sb, ss, sh;
+};
+
+struct Args {
+  View q, k, v, dout;
+  void *out, *dq, *dk, *dv;    // contiguous; out is read by backward
+  float *lse, *delta;          // [b, hk, sq*g]; lse in base 2 of scaled scores
+  const void *q_lens, *kv_lens;  // [b] int32 / int64, or null
+  int lens64;
+  int b, sq, sk, hk, g, hd, causal;
+  unsigned g_mul;
+  int g_shift;
+  float scale;
+};
+
+__device__ const uint4 kZeros = {0, 0, 0, 0};
+__device__ const float kInf = INFINITY;
+
+DEV_INLINE int length_of(const void* lens, int wide, int b, int most) {
+  if (!lens) return most;
+  long n = wide ? reinterpret_cast<const long*>(lens)[b]
+                : (long)reinterpret_cast<const int*>(lens)[b];
+  return n < 0 ? 0 : n > most ? most : (int)n;
+}
+
+// one block's sequence and key head
+struct Seq {
+  int batch, kvh, qlen, klen, off;  // off = klen - qlen
+  int rows;                         // qlen * g
+  DEV_INLINE Seq(const Args& a, int bh) {
+    batch = bh / a.hk;
+    kvh = bh - batch * a.hk;
+    qlen = length_of(a.q_lens, a.lens64, batch, a.sq);
+    klen = length_of(a.kv_lens, a.lens64, batch, a.sk);
+    off = klen - qlen;
+    rows = qlen * a.g;
+  }
+};
+
+template <int HDT> struct Geo {
+  static constexpr int NCH = HDT == 64 ? 8 : 16;  // chunks of an LDS row
+  static constexpr int PITCH = NCH * 16;
+  static constexpr int KS = HDT / 16;  // k steps of a product over the head
+  static constexpr int DT = HDT / 32;  // 32-column tiles of the head
+  static constexpr int BYTES = TILE * PITCH;
+};
+
+DEV_INLINE int perm(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+
+// A or B operand whose k runs along the row: rows r0 + (lane & 31), elements
+// 16*ks + 8*(lane >> 5) + 0..7
+template <int HDT>
+DEV_INLINE s16x8 frag_row(const char* lds, int r0, int ks, int lane) {
+  return *reinterpret_cast<const s16x8*>(
+      lds + (r0 + (lane & 31)) * Geo<HDT>::PITCH +
+      (((2 * ks + (lane >> 5)) ^ perm(lane)) << 4));
+}
+
+// A operand whose k runs down the rows, in the accumulators' order: column
+// 32*dt + (lane & 31), rows r0 + 4*h + 0..3 and r0 + 8 + 4*h + 0..3 with
+// h = lane >> 5. The transposing read hands each lane of 16 one column of
+// the 4 x 16 block that the 16 lanes fetch in 8-byte pieces.
+template <int HDT>
+DEV_INLINE s16x8 frag_col(const char* lds, int r0, int dt, int lane) {
+  int row = 4 * (lane >> 5) + ((lane >> 2) & 3);
+  int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1);
+  const char* p = lds + (r0 + row) * Geo<HDT>::PITCH +
+                  ((chunk ^ perm(row)) << 4) + (lane & 1) * 8;
+  typedef __attribute__((address_space(3))) s16x4* tp_t;
+  s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tp_t)p);
+  s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (tp_t)(p + 8 * Geo<HDT>::PITCH));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+typedef const __attribute__((address_space(1))) uint32_t* gp_t;
+typedef __attribute__((address_space(3))) uint32_t* lp_t;
+// global to LDS: lane l's 16 (4) bytes land at dst + 16 (4) * l
+DEV_INLINE void to_lds16(const void* src, void* dst) {
+  __builtin_amdgcn_global_load_lds((gp_t)src, (lp_t)dst, 16, 0, 0);
+}
+DEV_INLINE void to_lds4(const void* src, void* dst) {
+  __builtin_amdgcn_global_load_lds((gp_t)src, (lp_t)dst, 4, 0, 0);
+}
+
+// Tile of 64 rows r0.. below `end` to LDS, by NW waves. PACKED: row r is
+// position r / g of head r % g, else position r.
+template <int HDT, int NW, bool PACKED>
+DEV_INLINE void stage(const Args& a, const char* base, long ss, long sh,
+                      int r0, int end, char* lds, int wave, int lane) {
+  constexpr int NCH = Geo<HDT>::NCH, RPI = 64 / NCH;
+#pragma unroll
+  for (int i = 0; i < TILE / RPI / NW; ++i) {
+    int idx = wave * (TILE / RPI / NW) + i;
+    int row = idx * RPI + lane / NCH;
+    int chunk = (lane % NCH) ^ perm(row);
+    int r = r0 + row;
+    long at;
+    if (PACKED) {
+      int pos = (int)mdiv(r, a.g_mul, a.g_shift);
+      at = pos * ss + (r - pos * a.g) * sh;
+    } else {
+      at = r * ss;
+    }
+    const char* src = base + 2 * (at + chunk * 8);
+    if (r >= end || chunk * 8 >= a.hd)
+      src = reinterpret_cast<const char*>(&kZeros);
+    to_lds16(src, lds + idx * 1024);
+  }
+}
+
+// the lane's row of a kept operand, in registers
+template <int HDT>
+DEV_INLINE void keep(const Args& a, const char* row, bool valid, int lane,
+                     s16x8* f) {
+#pragma unroll
+  for (int ks = 0; ks < Geo<HDT>::KS; ++ks) {
+    int e = ks * 16 + (lane >> 5) * 8;
+    s16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+    f[ks] = valid && e < a.hd
+                ? *reinterpret_cast<const s16x8*>(row + 2 * e)
+                : z;
+  }
+}
+
+// accumulators acc[DT] (lane: one row, d = 32*dt + 8*j + 4*h + 0..3) times m
+// to the row's memory, 8 bytes a piece
+template <typename T, int DT>
+DEV_INLINE void put_row(T* row, const f32x16* acc, float m, int hd, int lane) {
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      int d = dt * 32 + j * 8 + (lane >> 5) * 4;
+      if (d < hd) {
+        uint2 v = {Op<T>::pack(acc[dt][4 * j] * m, acc[dt][4 * j + 1] * m),
+                   Op<T>::pack(acc[dt][4 * j + 2] * m,
+                               acc[dt][4 * j + 3] * m)};
+        *reinterpret_cast<uint2*>(row + d) = v;
+      }
+    }
+}
+
+DEV_INLINE float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+DEV_INLINE s16x8 pack8(const unsigned* p) {
+  uint4 v = {p[0], p[1], p[2], p[3]};
+  return __builtin_bit_cast(s16x8, v);
+}
+
+DEV_INLINE void staged() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+DEV_INLINE int wave_min(int x) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) {
+    int o = __shfl_xor(x, m, 64);
+    x = x < o ? x : o;
+  }
+  return __builtin_amdgcn_readfirstlane(x);
+}
+DEV_INLINE int wave_max(int x) { return -wave_min(-x); }
+
+constexpr f32x16 kNone = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+
+// a lane's row of the packed rows and how many keys it sees
+struct Row {
+  int r, pos, head, lim;
+  bool valid, stored;
+  DEV_INLINE Row(const Args& a, const Seq& s, int row) {
+    r = row;
+    pos = (int)mdiv(r, a.g_mul, a.g_shift);
+    head = s.kvh * a.g + (r - pos * a.g);
+    stored = pos < a.sq;
+    valid = pos < s.qlen;
+    lim = s.klen;
+    if (a.causal && valid) {
+      lim = pos + s.off + 1;
+      lim = lim < 0 ? 0 : lim;  // pos < qlen keeps it <= klen
+    }
+  }
+};
+
+// ---- forward: a block has 128 packed rows, a wave 32 ----------------------
+template <typename T, int HDT>
+__global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk) {
+  using G = Geo<HDT>;
+  __shared__ __attribute__((aligned(16))) char ktile[2][G::BYTES];
+  __shared__ __attribute__((aligned(16))) char vtile[2][G::BYTES];
+  int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  int bh = blockIdx.x / nblk;
+  int blk = nblk - 1 - (blockIdx.x - bh * nblk);  // longest rows first
+  Seq s(a, bh);
+  Row row(a, s, blk * 128 + wave * 32 + (lane & 31));
+  const char* kb = reinterpret_cast<const char*>(a.k.p) +
+                   2 * (s.batch * a.k.sb + s.kvh * a.k.sh);
+  const char* vb = reinterpret_cast<const char*>(a.v.p) +
+                   2 * (s.batch * a.v.sb + s.kvh * a.v.sh);
+  s16x8 qf[G::KS];
+  keep<HDT>(a,
+            reinterpret_cast<const char*>(a.q.p) +
+                2 * (s.batch * a.q.sb + row.pos * a.q.ss + row.head * a.q.sh),
+            row.valid, lane, qf);
+  // keys that any row of the block sees: the last row's, or none
+  int last = (blk * 128 + 127) / a.g;
+  last = last < s.qlen ? last : s.qlen - 1;
+  int end = blk * 128 < s.rows ? s.klen : 0;
+  if (a.causal && last + s.off + 1 < end) end = last + s.off + 1;
+  int ntile = end > 0 ? (end + TILE - 1) / TILE : 0;
+  int wlo = wave_min(row.lim), whi = wave_max(row.valid ? row.lim : 0);
+
+  float c = a.scale * kLog2e, far = 8.f / c;
+  float top = -INFINITY, sum = 0.f;
+  f32x16 acc[G::DT];
+#pragma unroll
+  for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
+
+  if (ntile) {
+    stage<HDT, 4, false>(a, kb, a.k.ss, 0, 0, s.klen, ktile[0], wave, lane);
+    stage<HDT, 4, false>(a, vb, a.v.ss, 0, 0, s.klen, vtile[0], wave, lane);
+  }
+  staged();
+  for (int t = 0; t < ntile; ++t) {
+    if (t + 1 < ntile) {
+      stage<HDT, 4, false>(a, kb, a.k.ss, 0, (t + 1) * TILE, s.klen,
+                           ktile[(t + 1) & 1], wave, lane);
+      stage<HDT, 4, false>(a, vb, a.v.ss, 0, (t + 1) * TILE, s.klen,
+                           vtile[(t + 1) & 1], wave, lane);
+    }
+    const char *kt = ktile[t & 1], *vt = vtile[t & 1];
+    int k0 = t * TILE;
+    if (k0 < whi) {
+      f32x16 sc[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        sc[u] = kNone;
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ++ks)
+          sc[u] = Op<T>::mfma(frag_row<HDT>(kt, u * 32, ks, lane), qf[ks],
+                              sc[u]);
+      }
+      if (k0 + TILE > wlo)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            int key = k0 + u * 32 + (i >> 2) * 8 + h * 4 + (i & 3);
+            sc[u][i] = key < row.lim ? sc[u][i] : -INFINITY;
+          }
+      float m = sc[0][0];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) m = fmaxf(m, sc[i >> 4][i & 15]);
+      m = fmaxf(m, other_half(m));
+      // P is taken relative to `top`, which follows the running maximum
+      // only when that is 2^8 past it: P stays below 2^8, which neither
+      // 16-bit type minds, and most steps rescale nothing
+      bool up = m > top + far;
+      if (__any(up)) {
+        float f = up ? __builtin_amdgcn_exp2f((top - m) * c) : 1.f;
+        top = up ? m : top;
+        sum *= f;
+#pragma unroll
+        for (int i = 0; i < G::DT; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[i][j] *= f;
+      }
+      float base = top == -INFINITY ? 0.f : -top * c;
+      unsigned p[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float x = __builtin_amdgcn_exp2f(
+            fmaf(sc[i >> 3][(2 * i) & 15], c, base));
+        float y = __builtin_amdgcn_exp2f(
+            fmaf(sc[i >> 3][(2 * i + 1) & 15], c, base));
+        sum += x + y;
+        p[i] = Op<T>::pack(x, y);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int i = 0; i < G::DT; ++i)
+          acc[i] = Op<T>::mfma(frag_col<HDT>(vt, k * 16, i, lane),
+                               pack8(p + 4 * k), acc[i]);
+    }
+    staged();
+  }
+  sum += other_half(sum);
+  if (!row.stored) return;
+  bool some = row.valid && row.lim > 0;
+  T* o = reinterpret_cast<T*>(a.out) +
+         (((long)s.batch * a.sq + row.pos) * a.hk * a.g + row.head) * a.hd;
+  if (!some)
+#pragma unroll
+    for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
+  put_row<T, G::DT>(o, acc, some ? 1.f / sum : 0.f, a.hd, lane);
+  if (h == 0 && a.lse)
+    a.lse[(long)bh * a.sq * a.g + row.r] =
+        some ? top * c + __builtin_amdgcn_logf(sum) : INFINITY;
+}
+
+// ---- backward 1: D, and dQ of 128 packed rows -----------------------------
+template <typename T, int HDT>
+__global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk) {
+  using G = Geo<HDT>;
+  __shared__ __attribute__((aligned(16))) char ktile[2][G::BYTES];
+  __shared__ __attribute__((aligned(16))) char vtile[2][G::BYTES];
+  int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  int bh = blockIdx.x / nblk;
+  int blk = nblk - 1 - (blockIdx.x - bh * nblk);
+  Seq s(a, bh);
+  Row row(a, s, blk * 128 + wave * 32 + (lane & 31));
+  const char* kb = reinterpret_cast<const char*>(a.k.p) +
+                   2 * (s.batch * a.k.sb + s.kvh * a.k.sh);
+  const char* vb = reinterpret_cast<const char*>(a.v.p) +
+                   2 * (s.batch * a.v.sb + s.kvh * a.v.sh);
+  int last = (blk * 128 + 127) / a.g;
+  last = last < s.qlen ? last : s.qlen - 1;
+  int end = blk * 128 < s.rows ? s.klen : 0;
+  if (a.causal && last + s.off + 1 < end) end = last + s.off + 1;
+  int ntile = end > 0 ? (end + TILE - 1) / TILE : 0;
+  int wlo = wave_min(row.lim), whi = wave_max(row.valid ? row.lim : 0);
+  if (ntile) {
+    stage<HDT, 4, false>(a, kb, a.k.ss, 0, 0, s.klen, ktile[0], wave, lane);
+    stage<HDT, 4, false>(a, vb, a.v.ss, 0, 0, s.klen, vtile[0], wave, lane);
+  }
+  s16x8 qf[G::KS], df[G::KS];
+  keep<HDT>(a,
+            reinterpret_cast<const char*>(a.dout.p) +
+                2 * (s.batch * a.dout.sb + row.pos * a.dout.ss +
+                     row.head * a.dout.sh),
+            row.valid, lane, df);
+  long oat = (((long)s.batch * a.sq + row.pos) * a.hk * a.g + row.head) *
+             a.hd;
+  // D from the stored output: its rounding moves dS by P times a sum of
+  // random half steps, below dS's own rounding
+  keep<HDT>(a, reinterpret_cast<const char*>(a.out) + 2 * oat, row.valid,
+            lane, qf);
+  float delta = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < G::KS; ++ks)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      T x = __builtin_bit_cast(T, (short)qf[ks][i]);
+      T y = __builtin_bit_cast(T, (short)df[ks][i]);
+      delta += to_f32(x) * to_f32(y);
+    }
+  delta += other_half(delta);
+  keep<HDT>(a,
+            reinterpret_cast<const char*>(a.q.p) +
+                2 * (s.batch * a.q.sb + row.pos * a.q.ss + row.head * a.q.sh),
+            row.valid, lane, qf);
+  float lse = INFINITY;
+  long lat = (long)bh * a.sq * a.g + row.r;
+  if (row.valid) lse = a.lse[lat];
+  if (row.stored && h == 0) a.delta[lat] = delta;
+
+  float c = a.scale * kLog2e;
+  f32x16 acc[G::DT];
+#pragma unroll
+  for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
+  staged();
+  for (int t = 0; t < ntile; ++t) {
+    if (t + 1 < ntile) {
+      stage<HDT, 4, false>(a, kb, a.k.ss, 0, (t + 1) * TILE, s.klen,
+                           ktile[(t + 1) & 1], wave, lane);
+      stage<HDT, 4, false>(a, vb, a.v.ss, 0, (t + 1) * TILE, s.klen,
+                           vtile[(t + 1) & 1], wave, lane);
+    }
+    const char *kt = ktile[t & 1], *vt = vtile[t & 1];
+    int k0 = t * TILE;
+    if (k0 < whi)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f32x16 sc = kNone, dp = kNone;
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ++ks)
+          sc = Op<T>::mfma(frag_row<HDT>(kt, u * 32, ks, lane), qf[ks], sc);
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ++ks)
+          dp = Op<T>::mfma(frag_row<HDT>(vt, u * 32, ks, lane), df[ks], dp);
+        if (k0 + u * 32 + 32 > wlo)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            int key = k0 + u * 32 + (i >> 2) * 8 + h * 4 + (i & 3);
+            sc[i] = key < row.lim ? sc[i] : -INFINITY;
+          }
+        unsigned p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float x = __builtin_amdgcn_exp2f(fmaf(sc[2 * i], c, -lse)) *
+                    (dp[2 * i] - delta);
+          float y = __builtin_amdgcn_exp2f(fmaf(sc[2 * i + 1], c, -lse)) *
+                    (dp[2 * i + 1] - delta);
+          p[i] = Op<T>::pack(x, y);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = 0; i < G::DT; ++i)
+            acc[i] = Op<T>::mfma(frag_col<HDT>(kt, u * 32 + k * 16, i, lane),
+                                 pack8(p + 4 * k), acc[i]);
+      }
+    staged();
+  }
+  if (!row.stored) return;
+  bool some = row.valid && row.lim > 0;
+  if (!some)
+#pragma unroll
+    for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
+  put_row<T, G::DT>(reinterpret_cast<T*>(a.dq) + oat, acc, a.scale, a.hd,
+                    lane);
+}
+
+// ---- backward 2: dK, dV of 128 keys, over all packed rows -----------------
+template <typename T, int HDT>
+__global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk) {
+  using G = Geo<HDT>;
+  __shared__ __attribute__((aligned(16))) char qtile[2][G::BYTES];
+  __shared__ __attribute__((aligned(16))) char dtile[2][G::BYTES];
+  __shared__ __attribute__((aligned(16))) float stat[2][2][TILE];
+  int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  int bh = blockIdx.x / nblk;
+  int blk = blockIdx.x - bh * nblk;  // the first keys are seen most
+  Seq s(a, bh);
+  int key = blk * 128 + wave * 32 + (lane & 31);
+  bool valid = key < s.klen;
+  s16x8 kf[G::KS], vf[G::KS];
+  keep<HDT>(a,
+            reinterpret_cast<const char*>(a.k.p) +
+                2 * (s.batch * a.k.sb + s.kvh * a.k.sh + key * a.k.ss),
+            valid, lane, kf);
+  keep<HDT>(a,
+            reinterpret_cast<const char*>(a.v.p) +
+                2 * (s.batch * a.v.sb + s.kvh * a.v.sh + key * a.v.ss),
+            valid, lane, vf);
+  const char* qb = reinterpret_cast<const char*>(a.q.p) +
+                   2 * (s.batch * a.q.sb + (long)s.kvh * a.g * a.q.sh);
+  const char* db = reinterpret_cast<const char*>(a.dout.p) +
+                   2 * (s.batch * a.dout.sb + (long)s.kvh * a.g * a.dout.sh);
+  const float* lse = a.lse + (long)bh * a.sq * a.g;
+  const float* del = a.delta + (long)bh * a.sq * a.g;
+  // rows from `lo` on see this lane's key
+  int lo = 0;
+  if (a.causal) lo = key > s.off ? (key - s.off) * a.g : 0;
+  int first = 0;
+  if (a.causal && blk * 128 > s.off) first = (blk * 128 - s.off) * a.g;
+  first &= ~(TILE - 1);
+  int ntile = 0;
+  if (blk * 128 < s.klen && first < s.rows)
+    ntile = (s.rows - first + TILE - 1) / TILE;
+  int wlo = wave_min(lo), whi = wave_max(valid ? lo : 0);
+  bool wlive = wave_max(valid) != 0;
+
+  auto load = [&](int t) {
+    int r0 = first + t * TILE, buf = t & 1;
+    stage<HDT, 4, true>(a, qb, a.q.ss, a.q.sh, r0, s.rows, qtile[buf], wave,
+                        lane);
+    stage<HDT, 4, true>(a, db, a.dout.ss, a.dout.sh, r0, s.rows, dtile[buf],
+                        wave, lane);
+    if (wave < 2) {
+      bool in = r0 + lane < s.rows;
+      const float* src = wave ? (in ? del + r0 + lane
+                                    : reinterpret_cast<const float*>(&kZeros))
+                              : (in ? lse + r0 + lane : &kInf);
+      to_lds4(src, stat[buf][wave]);
+    }
+  };
+  float c = a.scale * kLog2e;
+  f32x16 dk[G::DT], dv[G::DT];
+#pragma unroll
+  for (int i = 0; i < G::DT; ++i) dk[i] = dv[i] = kNone;
+  if (ntile) load(0);
+  staged();
+  for (int t = 0; t < ntile; ++t) {
+    if (t + 1 < ntile) load(t + 1);
+    const char *qt = qtile[t & 1], *dt = dtile[t & 1];
+    const float *ls = stat[t & 1][0], *ds = stat[t & 1][1];
+    int r0 = first + t * TILE;
+    if (wlive && r0 + TILE > wlo)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f32x16 sc = kNone, dp = kNone;
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ++ks)
+          sc = Op<T>::mfma(frag_row<HDT>(qt, u * 32, ks, lane), kf[ks], sc);
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ++ks)
+          dp = Op<T>::mfma(frag_row<HDT>(dt, u * 32, ks, lane), vf[ks], dp);
+        if (r0 + u * 32 < whi)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            int r = r0 + u * 32 + (i >> 2) * 8 + h * 4 + (i & 3);
+            sc[i] = r >= lo ? sc[i] : -INFINITY;
+          }
+        unsigned p[8], d[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float4 l4 = *reinterpret_cast<const float4*>(ls + u * 32 + j * 8 +
+                                                       h * 4);
+          float4 d4 = *reinterpret_cast<const float4*>(ds + u * 32 + j * 8 +
+                                                       h * 4);
+          const float *lp = &l4.x, *dl = &d4.x;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float x = __builtin_amdgcn_exp2f(
+                fmaf(sc[4 * j + 2 * i], c, -lp[2 * i]));
+            float y = __builtin_amdgcn_exp2f(
+                fmaf(sc[4 * j + 2 * i + 1], c, -lp[2 * i + 1]));
+            p[2 * j + i] = Op<T>::pack(x, y);
+            d[2 * j + i] = Op<T>::pack(x * (dp[4 * j + 2 * i] - dl[2 * i]),
+                                       y * (dp[4 * j + 2 * i + 1] -
+                                            dl[2 * i + 1]));
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = 0; i < G::DT; ++i) {
+            dv[i] = Op<T>::mfma(frag_col<HDT>(dt, u * 32 + k * 16, i, lane),
+                                pack8(p + 4 * k), dv[i]);
+            dk[i] = Op<T>::mfma(frag_col<HDT>(qt, u * 32 + k * 16, i, lane),
+                                pack8(d + 4 * k), dk[i]);
+          }
+      }
+    staged();
+  }
+  if (key >= a.sk) return;
+  if (!valid)
+#pragma unroll
+    for (int i = 0; i < G::DT; ++i) dk[i] = dv[i] = kNone;
+  long at = (((long)s.batch * a.sk + key) * a.hk + s.kvh) * a.hd;
+  put_row<T, G::DT>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, a.hd, lane);
+  put_row<T, G::DT>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, a.hd, lane);
+}
+
+template <typename T, int HDT>
+void launch(const Args& a, int bwd, hipStream_t s) {
+  int rblk = (a.sq * a.g + 127) / 128, kblk = (a.sk + 127) / 128;
+  int bh = a.b * a.hk;
+  if (!bwd) {
+    if (rblk) attn_rc_fwd_k<T, HDT><<<bh * rblk, 256, 0, s>>>(a, rblk);
+    return;
+  }
+  if (rblk) attn_rc_dq_k<T, HDT><<<bh * rblk, 256, 0, s>>>(a, rblk);
+  if (kblk) attn_rc_dkv_k<T, HDT><<<bh * kblk, 256, 0, s>>>(a, kblk);
+}
+
+}  // namespace
+
+extern "C" {
+
+// strides: q, k, v, dout, each (b, s, head) in elements; multiples of 8, all
+// pointers 16-byte aligned, hd a multiple of 8 up to 128. lens null or [b].
+// Forward writes out and, unless null, lse; backward reads both and writes
+// delta, dq, dk, dv. Grids must stay below 2^31 blocks and sq*g below 2^31.
+void pdta_attn_recompute(const void* q, const void* k, const void* v,
+                         const void* dout, const long* st, void* out,
+                         float* lse, float* delta, void* dq, void* dk,
+                         void* dv, const void* q_lens, const void* kv_lens,
+                         int lens64, int b, int sq, int sk, int hk, int g,
+                         int hd, float scale, int causal, int bwd, int dt,
+                         hipStream_t s) {
+  Args a;
+  a.q = {q, st[0], st[1], st[2]};
+  a.k = {k, st[3], st[4], st[5]};
+  a.v = {v, st[6], st[7], st[8]};
+  a.dout = {dout, st[9], st[10], st[11]};
+  a.out = out, a.dq = dq, a.dk = dk, a.dv = dv, a.lse = lse, a.delta = delta;
+  a.q_lens = q_lens, a.kv_lens = kv_lens, a.lens64 = lens64;
+  a.b = b, a.sq = sq, a.sk = sk, a.hk = hk, a.g = g, a.hd = hd;
+  a.scale = scale, a.causal = causal;
+  MagicDiv m = magic_div((unsigned)g);
+  a.g_mul = m.mul, a.g_shift = m.shift;
+  if (b == 0 || hk == 0) return;
+  PDTA_DISPATCH_DTYPE16(dt, T, {
+    if (hd <= 64)
+      launch<T, 64>(a, bwd, s);
+    else if (hd <= 96)
+      launch<T, 96>(a, bwd, s);
+    else
+      launch<T, 128>(a, bwd, s);
+  });
+}
+
+}  // extern "C"

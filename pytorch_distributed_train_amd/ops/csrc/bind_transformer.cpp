@@ -1,5 +1,5 @@
-// Python binding of the transformer-training operators (AdamW,
-// query/key norm with rotation).
+// Python binding of the transformer-training operators: AdamW,
+// query/key norm with rotation, attention with recomputed probabilities.
 // Arguments are checked here, before a launch: a kernel's bounds rest on them.
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
@@ -7,6 +7,7 @@
 
 #include <hip/hip_runtime_api.h>
 
+#include <cmath>
 #include <vector>
 
 extern "C" {
@@ -19,6 +20,10 @@ void pdta_qknorm(const void* const*, const long*, const void* const*,
                  const float*, const float*, const void*, int, int, int, int,
                  long, long, float, int, int, int, float*, float*, float*,
                  int, hipStream_t);
+void pdta_attn_recompute(const void*, const void*, const void*, const void*,
+                         const long*, void*, float*, float*, void*, void*,
+                         void*, const void*, const void*, int, int, int, int,
+                         int, int, int, float, int, int, int, hipStream_t);
 }
 
 namespace {
@@ -236,6 +241,148 @@ std::vector<at::Tensor> qk_norm_rope(
   return {y[0], y[1], dwq, dwk};
 }
 
+// ---- attention with recomputed probabilities -----------------------------
+struct AttnShape {
+  long b, sq, sk, h, hk, hd;
+};
+
+AttnShape attn_check(const at::Tensor& q, const at::Tensor& k,
+                     const at::Tensor& v,
+                     const c10::optional<at::Tensor>& q_lens,
+                     const c10::optional<at::Tensor>& kv_lens, double scale) {
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4,
+              "q, k and v must be [b, s, heads, hd]");
+  AttnShape n = {q.size(0), q.size(1), k.size(1),
+                 q.size(2), k.size(2), q.size(3)};
+  TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == n.b &&
+                  k.size(3) == n.hd,
+              "k and v must be [", n.b, ", sk, hk, ", n.hd, "]");
+  TORCH_CHECK(n.hd >= 8 && n.hd <= 128 && n.hd % 8 == 0,
+              "head size must be a multiple of 8 up to 128, is ", n.hd);
+  TORCH_CHECK(n.hk > 0 ? n.h % n.hk == 0 : n.h == 0, "heads of q (", n.h,
+              ") must be a multiple of those of k (", n.hk, ")");
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 ||
+                  q.scalar_type() == at::kHalf,
+              "q must be bfloat16 or float16 on GPU, is ", q.scalar_type());
+  for (const at::Tensor* t : {&q, &k, &v}) {
+    TORCH_CHECK(t->device() == q.device() &&
+                    t->scalar_type() == q.scalar_type(),
+                "q, k and v must have one device and dtype");
+    TORCH_CHECK(t->numel() == 0 || (t->stride(3) == 1 && rows8(*t)),
+                "rows must be contiguous, 16-byte aligned, strides "
+                "multiples of 8");
+  }
+  long g = n.hk ? n.h / n.hk : 1;
+  TORCH_CHECK((n.sq + n.sk + 1024) * g < (1l << 31) &&
+                  n.b * n.hk * ((n.sq * g + n.sk) / 128 + 2) < (1l << 31),
+              "attention: too many rows");
+  for (const auto* l : {&q_lens, &kv_lens})
+    if (l->has_value()) {
+      const at::Tensor& t = **l;
+      TORCH_CHECK(t.device() == q.device() && t.is_contiguous() &&
+                      t.numel() == n.b &&
+                      (t.scalar_type() == at::kInt ||
+                       t.scalar_type() == at::kLong),
+                  "lengths must be contiguous int32 or int64 [", n.b, "] on ",
+                  q.device());
+    }
+  if (q_lens.has_value() && kv_lens.has_value())
+    TORCH_CHECK(q_lens->scalar_type() == kv_lens->scalar_type(),
+                "q_lens and kv_lens must have one dtype");
+  TORCH_CHECK(scale > 0.0 && std::isfinite((float)scale) &&
+                  (float)scale > 0.f,
+              "scale must be positive, is ", scale);
+  return n;
+}
+
+void attn_strides(const at::Tensor& t, long* st) {
+  // a dimension of one element is never stepped along
+  for (int d = 0; d < 3; ++d) st[d] = t.size(d) > 1 ? t.stride(d) : 0;
+}
+
+const void* len_ptr(const c10::optional<at::Tensor>& t) {
+  return t.has_value() ? t->data_ptr() : nullptr;
+}
+
+bool lens_wide(const c10::optional<at::Tensor>& a,
+               const c10::optional<at::Tensor>& b) {
+  const auto& t = a.has_value() ? a : b;
+  return t.has_value() && t->scalar_type() == at::kLong;
+}
+
+// {out [b, sq, h, hd], lse [b, hk, sq * h / hk] (empty unless want_lse)}
+std::vector<at::Tensor> attn_recompute_fwd(
+    at::Tensor q, at::Tensor k, at::Tensor v,
+    c10::optional<at::Tensor> q_lens, c10::optional<at::Tensor> kv_lens,
+    double scale, bool causal, bool want_lse) {
+  TORCH_CHECK(q.is_cuda(), "q must be on GPU");
+  c10::DeviceGuard guard(q.device());
+  AttnShape n = attn_check(q, k, v, q_lens, kv_lens, scale);
+  long g = n.hk ? n.h / n.hk : 1;
+  auto out = at::empty({n.b, n.sq, n.h, n.hd}, q.options());
+  auto lse = at::empty({want_lse ? n.b * n.hk * n.sq * g : 0},
+                       q.options().dtype(at::kFloat));
+  long st[12] = {0};
+  attn_strides(q, st);
+  attn_strides(k, st + 3);
+  attn_strides(v, st + 6);
+  if (out.numel()) {
+    pdta_attn_recompute(q.data_ptr(), k.data_ptr(), v.data_ptr(), nullptr,
+                        st, out.data_ptr(),
+                        want_lse ? lse.data_ptr<float>() : nullptr, nullptr,
+                        nullptr, nullptr, nullptr, len_ptr(q_lens),
+                        len_ptr(kv_lens), lens_wide(q_lens, kv_lens), n.b,
+                        n.sq, n.sk, n.hk, g, n.hd, (float)scale, causal, 0,
+                        dt_of(q), cur_stream());
+    launched("attn_recompute_fwd");
+  }
+  return {out, lse};
+}
+
+// {dq, dk, dv}, contiguous
+std::vector<at::Tensor> attn_recompute_bwd(
+    at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor lse,
+    at::Tensor dout, c10::optional<at::Tensor> q_lens,
+    c10::optional<at::Tensor> kv_lens, double scale, bool causal) {
+  TORCH_CHECK(q.is_cuda(), "q must be on GPU");
+  c10::DeviceGuard guard(q.device());
+  AttnShape n = attn_check(q, k, v, q_lens, kv_lens, scale);
+  long g = n.hk ? n.h / n.hk : 1;
+  for (const at::Tensor* t : {&out, &dout})
+    TORCH_CHECK(t->device() == q.device() &&
+                    t->scalar_type() == q.scalar_type() &&
+                    t->sizes() == q.sizes(),
+                "out and its gradient must be like q");
+  TORCH_CHECK(out.is_contiguous() &&
+                  (dout.numel() == 0 || (dout.stride(3) == 1 && rows8(dout))),
+              "out must be contiguous, its gradient have aligned rows");
+  TORCH_CHECK(lse.device() == q.device() &&
+                  lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+                  lse.numel() == n.b * n.hk * n.sq * g,
+              "lse must be the forward's");
+  auto dq = at::empty({n.b, n.sq, n.h, n.hd}, q.options());
+  auto dk = at::empty({n.b, n.sk, n.hk, n.hd}, q.options());
+  auto dv = at::empty_like(dk);
+  auto delta = at::empty_like(lse);
+  long st[12];
+  attn_strides(q, st);
+  attn_strides(k, st + 3);
+  attn_strides(v, st + 6);
+  attn_strides(dout, st + 9);
+  if (dq.numel() || dk.numel()) {
+    pdta_attn_recompute(q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                        dout.data_ptr(), st, out.data_ptr(),
+                        lse.data_ptr<float>(), delta.data_ptr<float>(),
+                        dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                        len_ptr(q_lens), len_ptr(kv_lens),
+                        lens_wide(q_lens, kv_lens), n.b, n.sq, n.sk, n.hk, g,
+                        n.hd, (float)scale, causal, 1, dt_of(q),
+                        cur_stream());
+    launched("attn_recompute_bwd");
+  }
+  return {dq, dk, dv};
+}
+
 }  // namespace
 
 void bind_transformer(pybind11::module_& m) {
@@ -249,4 +396,11 @@ void bind_transformer(pybind11::module_& m) {
         py::arg("sin"), py::arg("positions"), py::arg("eps"),
         py::arg("interleaved"), py::arg("dq") = py::none(),
         py::arg("dk") = py::none());
+  m.def("attn_recompute_fwd", &attn_recompute_fwd, py::arg("q"),
+        py::arg("k"), py::arg("v"), py::arg("q_lens"), py::arg("kv_lens"),
+        py::arg("scale"), py::arg("causal"), py::arg("want_lse"));
+  m.def("attn_recompute_bwd", &attn_recompute_bwd, py::arg("q"),
+        py::arg("k"), py::arg("v"), py::arg("out"), py::arg("lse"),
+        py::arg("dout"), py::arg("q_lens"), py::arg("kv_lens"),
+        py::arg("scale"), py::arg("causal"));
 }

@@ -894,6 +894,149 @@ def attention_qkv(qkv2d, b, s, h, hd, nvalid, scale):
 
 
 # ---------------------------------------------------------------------------
+# Attention with recomputed probabilities
+# ---------------------------------------------------------------------------
+
+def _rows8(x):
+    """x [b, s, h, hd] itself if 16-byte accesses can walk its rows."""
+    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(
+            x.shape[d] <= 1 or x.stride(d) % 8 == 0 for d in range(3)):
+        return x
+    return x.contiguous()
+
+
+def _visible(q, k, causal, q_lens, kv_lens):
+    """[b, 1, 1, sq, sk] where a query may see a key, for the CPU path."""
+    sq, sk = q.shape[1], k.shape[1]
+    i, j = torch.arange(sq)[:, None], torch.arange(sk)[None, :]
+    at = (-1, 1, 1, 1, 1)
+    ql = torch.tensor([sq]) if q_lens is None else q_lens.long().clamp(0, sq)
+    kl = torch.tensor([sk]) if kv_lens is None \
+        else kv_lens.long().clamp(0, sk)
+    ql, kl = ql.view(at), kl.view(at)
+    ok = (i < ql) & (j < kl)
+    if causal:
+        ok = ok & (j <= i + kl - ql)
+    return ok
+
+
+class AttentionRecomputeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, causal, q_lens, kv_lens):
+        ctx.scale, ctx.causal = scale, causal
+        if q.is_cuda:
+            q, k, v = _rows8(q), _rows8(k), _rows8(v)
+            out, lse = ext().attn_recompute_fwd(
+                q, k, v, q_lens, kv_lens, scale, causal,
+                any(ctx.needs_input_grad))
+            ctx.save_for_backward(q, k, v, out, lse, q_lens, kv_lens)
+            return out
+        b, sq, h, hd = q.shape
+        hk = k.shape[2]
+        ok = _visible(q, k, causal, q_lens, kv_lens)
+        # what is masked may hold anything: 0 * inf must not come up
+        seen_k = ok.any(3)[:, 0, 0, :, None, None]
+        seen_q = ok.any(4)[:, 0, 0, :, None, None]
+        q5, k5, v5 = (_heads_first(_wide(x).masked_fill(~m, 0.0), hk)
+                      for x, m in ((q, seen_q), (k, seen_k), (v, seen_k)))
+        s = (q5 @ k5.transpose(-1, -2)) * scale
+        lse = s.masked_fill(~ok, float("-inf")).logsumexp(-1, keepdim=True)
+        lse = lse.masked_fill(lse == float("-inf"), float("inf"))
+        p = (s - lse).exp().masked_fill(~ok, 0.0)
+        out = _heads_last(p @ v5, h).to(q.dtype)
+        ctx.save_for_backward(q, k, v, out, lse, q_lens, kv_lens)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse, q_lens, kv_lens = ctx.saved_tensors
+        scale, causal = ctx.scale, ctx.causal
+        if q.is_cuda:
+            dq, dk, dv = ext().attn_recompute_bwd(
+                q, k, v, out, lse, _rows8(dout), q_lens, kv_lens, scale,
+                causal)
+            return dq, dk, dv, None, None, None, None
+        h, hk = q.shape[2], k.shape[2]
+        ok = _visible(q, k, causal, q_lens, kv_lens)
+        seen_k = ok.any(3)[:, 0, 0, :, None, None]
+        seen_q = ok.any(4)[:, 0, 0, :, None, None]
+        q5, k5, v5, o5, g5 = (
+            _heads_first(_wide(x).masked_fill(~m, 0.0), hk)
+            for x, m in ((q, seen_q), (k, seen_k), (v, seen_k),
+                         (out, seen_q), (dout, seen_q)))
+        p = ((q5 @ k5.transpose(-1, -2)) * scale - lse).exp() \
+            .masked_fill(~ok, 0.0)
+        dv = (p.transpose(-1, -2) @ g5).sum(2, keepdim=True)
+        ds = p * (g5 @ v5.transpose(-1, -2)
+                  - (g5 * o5).sum(-1, keepdim=True)) * scale
+        dq = _heads_last(ds @ k5, h).to(q.dtype)
+        dk = (ds.transpose(-1, -2) @ q5).sum(2, keepdim=True)
+        return (dq, _heads_last(dk, hk).to(k.dtype),
+                _heads_last(dv, hk).to(v.dtype), None, None, None, None)
+
+
+def _heads_first(x, hk):
+    # [b, s, h, hd] -> [b, hk, h/hk, s, hd]
+    b, s, h, hd = x.shape
+    return x.view(b, s, hk, h // hk, hd).permute(0, 2, 3, 1, 4)
+
+
+def _heads_last(x, h):
+    b, _, _, s, hd = x.shape
+    return x.permute(0, 3, 1, 2, 4).reshape(b, s, h, hd)
+
+
+def attention_recompute(q, k, v, scale: float | None = None,
+                        causal: bool = False, q_lens=None, kv_lens=None):
+    """softmax(scale q k^T) v without an sq x sk tensor in either direction:
+    the forward keeps each row's log-sum-exp, the backward recomputes the
+    probabilities from it. Returns [b, sq, h, hd], contiguous.
+
+    q [b, sq, h, hd], k, v [b, sk, hk, hd]; h a multiple of hk: h/hk
+    neighbouring query heads share a key head. Any strides (the views of one
+    projection's output need no copy when their rows are 16-byte aligned).
+    scale: positive, None for 1/sqrt(hd).
+    q_lens, kv_lens: int32 or int64 [b], the sequences' lengths (None: sq,
+    sk); cut to 0..sq, 0..sk. What lies behind them is never read; outputs
+    and gradients there are 0.
+    causal: query i sees keys up to i + kv_len - q_len, so the last query
+    sees the last key. A query that sees none gives 0.
+    GPU (csrc/attn_recompute.hip): bf16 and fp16, hd a multiple of 8 up to
+    128; one launch forward, two backward; results do not depend on timing.
+    In fp16, gradients need a loss scale that keeps dS in its range, as the
+    fp16 training path has."""
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape \
+            or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError("q must be [b, sq, h, hd], k and v [b, sk, hk, hd]: "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    b, h, hk, hd = q.shape[0], q.shape[2], k.shape[2], q.shape[3]
+    if hk == 0 or h % hk or hd == 0:
+        raise ValueError(f"{h} query heads for {hk} key heads of {hd}")
+    if not q.dtype == k.dtype == v.dtype \
+            or not q.device == k.device == v.device:
+        raise ValueError("q, k and v must have one dtype and device")
+    if q.is_cuda and (hd % 8 or hd > 128):
+        raise ValueError(f"head size must be a multiple of 8 up to 128: {hd}")
+    if scale is None:
+        scale = hd ** -0.5
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive: {scale}")
+    for x in (q_lens, kv_lens):
+        if x is not None and (x.shape != (b,) or x.device != q.device
+                              or x.dtype not in (torch.int32, torch.int64)):
+            raise ValueError(f"lengths must be int32 or int64 [{b}] on "
+                             f"{q.device}")
+    if q_lens is not None and kv_lens is not None \
+            and q_lens.dtype != kv_lens.dtype:
+        q_lens, kv_lens = q_lens.long(), kv_lens.long()
+    q_lens, kv_lens = (x if x is None else x.contiguous()
+                       for x in (q_lens, kv_lens))
+    return AttentionRecomputeFn.apply(q, k, v, float(scale), bool(causal),
+                                      q_lens, kv_lens)
+
+
+# ---------------------------------------------------------------------------
 # Query/key norm with the position rotation
 # ---------------------------------------------------------------------------
 

@@ -1,0 +1,353 @@
+"""Attention with recomputed probabilities: forward and gradients against
+the definition in 64 bits with bounds from its roundings, masks that leave
+rows empty, lengths, heads, strides, and refusals."""
+import math
+
+import pytest
+import torch
+
+from pytorch_distributed_train_amd.ops import functional as OF
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def _lens(x, b, most):
+    return [most] * b if x is None else \
+        [min(max(int(i), 0), most) for i in x]
+
+
+def _oracle(q, k, v, dout, scale, causal, q_lens, kv_lens):
+    """(out, dq, dk, dv) in 64 bits, and how far a kernel may be off that
+    works in fp32 and rounds P, dS, the output and the gradients to the
+    tensors' type once each."""
+    half = torch.finfo(q.dtype).eps / 2
+    # fp16 values below 2^-14 are off by half of the least step instead;
+    # bf16 and fp32 have their least normal number at 2^-126, and a
+    # probability below it (exp of less than -87.3) may come out as 0: off
+    # by itself, so by less than 2^-126
+    least = 2.0 ** -25 if q.dtype == torch.float16 else 2.0 ** -126
+    hd, g = q.shape[3], q.shape[2] // k.shape[2]
+    Q, K, V, DO = (x.detach().double().cpu() for x in (q, k, v, dout))
+    val = [torch.zeros_like(Q), torch.zeros_like(Q), torch.zeros_like(K),
+           torch.zeros_like(K)]
+    err = [torch.zeros_like(x) for x in val]
+    ql = _lens(q_lens, Q.shape[0], Q.shape[1])
+    kl = _lens(kv_lens, K.shape[0], K.shape[1])
+    for b, (m, n) in enumerate(zip(ql, kl)):
+        ok = torch.ones(m, n, dtype=torch.bool)
+        if causal:
+            ok = torch.arange(n)[None] <= torch.arange(m)[:, None] + n - m
+        rows = ok.any(1)
+        for h in range(Q.shape[2]):
+            if m == 0 or n == 0:
+                continue
+            a, kk, vv, do = (Q[b, :m, h], K[b, :n, h // g],
+                             V[b, :n, h // g], DO[b, :m, h])
+            s = (a @ kk.t()) * scale
+            p = torch.zeros_like(s)
+            p[rows] = torch.softmax(
+                s[rows].masked_fill(~ok[rows], float("-inf")), -1)
+            o = p @ vv
+            dp = do @ vv.t()
+            ds = p * (dp - (do * o).sum(-1, keepdim=True))
+            val[0][b, :m, h] = o
+            val[1][b, :m, h] = ds @ kk * scale
+            val[2][b, :n, h // g] += ds.t() @ a * scale
+            val[3][b, :n, h // g] += p.t() @ do
+            # relative error of P: the scores' (hd + 16 fp32 roundings of
+            # the products' sum), the logarithm's, exp's, and in the sum
+            # over n keys
+            absum = (a.abs() @ kk.abs().t()) * scale
+            e = 2 * (hd + 16) * U * absum.masked_fill(~ok, 0).amax(
+                1, keepdim=True) * 2 + 64 * U + n * U
+            h_ = half + e
+            av = p @ vv.abs()
+            err[0][b, :m, h] = (h_ + 2 * e) * av + half * o.abs() \
+                + least * vv.abs().sum(0) + least
+            # D from the rounded output; dP's own sum
+            e_d = ((do.abs() * ((h_ + 2 * e) * av + half * o.abs()
+                                + least * vv.abs().sum(0) + least))
+                   .sum(-1, keepdim=True)
+                   + 2 * (hd + 16) * U * (do.abs() @ vv.abs().t()))
+            e_s = ds.abs() * h_ * 2 + p * (1 + e) * e_d + least
+            # accumulating m rows (n keys) in fp32
+            err[1][b, :m, h] = ((e_s + n * U * ds.abs()) @ kk.abs()) * scale \
+                + half * val[1][b, :m, h].abs() + least
+            err[2][b, :n, h // g] += ((e_s + g * m * U * ds.abs()).t()
+                                      @ a.abs()) * scale
+            err[3][b, :n, h // g] += (p * (h_ + g * m * U) + least).t() \
+                @ do.abs()
+    for i in (2, 3):
+        err[i] += half * val[i].abs() + least
+    return val, err
+
+
+def _check(got, val, err):
+    for x, w, e, what in zip(got, val, err, ("out", "dq", "dk", "dv")):
+        off = (x.detach().double().cpu() - w).abs()
+        # the rounding's own bound at a value that is off
+        bad = ~(off <= e * (1 + 2.0 ** -6))
+        assert not bool(bad.any()), \
+            f"{what}: {int(bad.sum())} of {bad.numel()} over the bound, " \
+            f"worst {float((off / e.clamp(min=1e-30)).max()):.3g} times"
+
+
+def _inputs(dev, dtype, b, sq, sk, h, hk, hd, seed=0, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+
+    def r(*s):
+        return (torch.randn(*s, generator=g) * std).to(dtype).to(dev)
+
+    return (r(b, sq, h, hd), r(b, sk, hk, hd), r(b, sk, hk, hd),
+            r(b, sq, h, hd))
+
+
+def _t(x, dev, dtype=torch.int32):
+    return None if x is None else torch.tensor(x, dtype=dtype, device=dev)
+
+
+def _run(q, k, v, dout, **kw):
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    out = OF.attention_recompute(*leaves, **kw)
+    return [out, *torch.autograd.grad(out, leaves, dout)]
+
+
+CASES = [
+    # b, sq, sk, h, hk, hd, causal, q_lens, kv_lens
+    (1, 1, 1, 1, 1, 64, False, None, None),
+    (2, 1, 300, 4, 2, 128, True, None, [300, 17]),
+    (2, 65, 65, 3, 3, 64, False, None, None),
+    (2, 197, 197, 2, 2, 64, False, None, None),
+    (1, 64, 64, 2, 1, 64, True, None, None),
+    (1, 63, 65, 2, 2, 64, False, None, None),
+    (1, 129, 127, 2, 2, 128, True, None, None),      # two rows see nothing
+    (2, 200, 90, 3, 1, 96, True, None, [90, 3]),     # most see nothing
+    (1, 130, 130, 6, 2, 128, True, None, None),      # three heads a key head
+    (1, 100, 333, 8, 1, 72, True, None, None),       # eight
+    (1, 77, 77, 5, 5, 8, False, None, None),
+    (1, 77, 140, 2, 2, 40, True, None, None),
+    (2, 150, 150, 2, 2, 104, False, None, None),
+    (2, 140, 140, 2, 1, 128, False, None, None),
+    (5, 150, 150, 2, 1, 80, False, [0, 1, 64, 149, 150],
+     [0, 1, 64, 149, 150]),
+    (5, 150, 150, 2, 2, 64, True, [0, 1, 64, 149, 150],
+     [0, 1, 64, 149, 150]),
+    (4, 70, 260, 4, 2, 128, False, [70, 0, 3, 69], [0, 260, 129, 1]),
+    (3, 40, 200, 4, 4, 64, True, [40, 7, 99], [-5, 200, 1000]),
+    (1, 700, 1100, 2, 1, 64, True, None, None),
+    (1, 1025, 1025, 4, 2, 128, True, None, None),
+    (3, 5, 2000, 2, 1, 128, True, None, [2000, 3, 777]),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_forward_backward(dtype, case):
+    b, sq, sk, h, hk, hd, causal, ql, kl = case
+    x = _inputs("cuda", dtype, b, sq, sk, h, hk, hd, seed=sq + hd)
+    want = _oracle(*x, hd ** -0.5, causal, ql, kl)
+    got = _run(*x, causal=causal, q_lens=_t(ql, "cuda"),
+               kv_lens=_t(kl, "cuda", torch.int32))
+    assert got[0].is_contiguous() and got[0].dtype == dtype
+    _check(got, *want)
+    again = _run(*x, causal=causal, q_lens=_t(ql, "cuda", torch.int64),
+                 kv_lens=_t(kl, "cuda", torch.int64))
+    for u, w in zip(got, again):
+        assert torch.equal(u, w), "two runs differ"
+    with torch.no_grad():  # without the row statistics
+        assert torch.equal(got[0], OF.attention_recompute(
+            *x[:3], causal=causal, q_lens=_t(ql, "cuda"),
+            kv_lens=_t(kl, "cuda")))
+
+
+@pytest.mark.parametrize("case", [c for c in CASES if c[1] <= 200], ids=str)
+def test_cpu_path(case):
+    """The CPU reference in fp32: under the bounds of a 16-bit kernel's
+    fp32 part, its P and dS unrounded."""
+    b, sq, sk, h, hk, hd, causal, ql, kl = case
+    x = _inputs("cpu", torch.float32, b, sq, sk, h, hk, hd, seed=sq + hd)
+    want = _oracle(*x, hd ** -0.5, causal, ql, kl)
+    _check(_run(*x, causal=causal, q_lens=_t(ql, "cpu"),
+                kv_lens=_t(kl, "cpu")), *want)
+
+
+@pytest.mark.parametrize("causal,ql,kl", [
+    (False, None, None), (True, None, None), (True, [3, 0], [2, 4]),
+    (False, [1, 4], [0, 5])])
+def test_gradients_against_differences(causal, ql, kl):
+    g = torch.Generator().manual_seed(2)
+    q = torch.randn(2, 4, 4, 3, generator=g, dtype=torch.float64)
+    k = torch.randn(2, 5, 2, 3, generator=g, dtype=torch.float64)
+    v = torch.randn(2, 5, 2, 3, generator=g, dtype=torch.float64)
+    assert torch.autograd.gradcheck(
+        lambda *a: OF.attention_recompute(
+            *a, scale=0.7, causal=causal, q_lens=_t(ql, "cpu"),
+            kv_lens=_t(kl, "cpu")),
+        [x.requires_grad_(True) for x in (q, k, v)], eps=1e-6, atol=1e-6)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"),
+                                 "lowest"])
+def test_what_lies_behind_a_sequence_is_not_read(dtype, bad):
+    if bad == "lowest":
+        bad = torch.finfo(dtype).min
+    b, s, h, hk, hd = 4, 150, 4, 2, 128
+    lens = [0, 1, 70, 129]
+    q, k, v, do = _inputs("cuda", dtype, b, s, s, h, hk, hd, seed=5)
+    want = _run(q, k, v, do, q_lens=_t(lens, "cuda"),
+                kv_lens=_t(lens, "cuda"))
+    for i, n in enumerate(lens):
+        for x in (q, k, v, do):
+            x[i, n:] = bad
+    got = _run(q, k, v, do, q_lens=_t(lens, "cuda"),
+               kv_lens=_t(lens, "cuda"))
+    for u, w in zip(got, want):
+        assert torch.equal(u, w)
+    for i, n in enumerate(lens):
+        for u in got:
+            assert bool((u[i, n:] == 0).all())
+
+
+@gpu
+def test_rising_and_far_scores():
+    """Maxima that rise by more and by less than 2^8 a step, and scores so
+    far apart that all but one probability vanish."""
+    for step in (0.001, 0.05, 3.0):
+        q, k, v, do = _inputs("cuda", torch.bfloat16, 1, 70, 700, 1, 1, 64,
+                              seed=8)
+        ramp = torch.arange(700, device="cuda", dtype=torch.float32) * step
+        k[0, :, 0, 0] = ramp.to(torch.bfloat16)
+        q[0, :, 0, 0] = 8.0
+        q[0, 35:, 0, 0] = -8.0  # and falling ones
+        want = _oracle(q, k, v, do, 0.125, False, None, None)
+        _check(_run(q, k, v, do), *want)
+
+
+@gpu
+def test_strides_offsets_and_broadcasts():
+    b, s, h, hk, hd = 2, 130, 4, 2, 64
+    # views of one projection's output, aligned and not
+    for pad in (0, 8, 3):
+        g = torch.Generator().manual_seed(pad)
+        qkv = torch.randn(b, s, (h + 2 * hk) * hd + pad, generator=g) \
+            .to(torch.bfloat16).cuda()
+        q, k, v = qkv[..., pad:].split([h * hd, hk * hd, hk * hd], -1)
+        q, k, v = (x.unflatten(-1, (-1, hd)) for x in (q, k, v))
+        do = torch.randn(h, b, s, hd, generator=g).to(torch.bfloat16).cuda() \
+            .permute(1, 2, 0, 3)
+        want = _run(*(x.contiguous() for x in (q, k, v, do)), causal=True)
+        for u, w in zip(_run(q, k, v, do, causal=True), want):
+            assert torch.equal(u, w), pad
+    # heads before positions, one sequence for all, the gradient of a sum
+    q, k, v, do = _inputs("cuda", torch.bfloat16, b, s, s, h, hk, hd)
+    qt = q.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+    ke, ve = k[:1].expand(b, -1, -1, -1), v[:1].expand(b, -1, -1, -1)
+    one = torch.ones(1, device="cuda", dtype=q.dtype).expand(q.shape)
+    want = _run(q, ke.contiguous(), ve.contiguous(), one.contiguous())
+    for u, w in zip(_run(qt, ke, ve, one), want):
+        assert torch.equal(u, w)
+    leaf = k[:1].clone().requires_grad_(True)
+    OF.attention_recompute(q, leaf.expand(b, -1, -1, -1), ve).backward(one)
+    assert torch.equal(leaf.grad, want[2].sum(0, keepdim=True))
+
+
+@gpu
+def test_offsets_past_32_bits():
+    """Two sequences more than 2^32 bytes apart in a long cache."""
+    far = (1 << 31) + (1 << 20)
+    big = torch.empty(far + (1 << 16), dtype=torch.bfloat16, device="cuda")
+    q, k, v, do = _inputs("cuda", torch.bfloat16, 2, 40, 40, 2, 2, 64)
+    views = []
+    for i, x in enumerate((q, k, v, do)):
+        at = big.as_strided(x.shape, (far, x.stride(1), x.stride(2), 1),
+                            i * 8192)
+        at.copy_(x)
+        views.append(at)
+    for u, w in zip(_run(*views), _run(q, k, v, do)):
+        assert torch.equal(u, w)
+
+
+@gpu
+def test_scale_and_empty():
+    q, k, v, do = _inputs("cuda", torch.float16, 1, 50, 60, 2, 2, 64)
+    want = _oracle(q, k, v, do, 0.31, False, None, None)
+    _check(_run(q, k, v, do, scale=0.31), *want)
+    for b, sq, sk in ((0, 5, 5), (2, 0, 5), (2, 5, 0)):
+        x = _inputs("cuda", torch.float16, b, sq, sk, 2, 1, 64)
+        for u, w in zip(_run(*x), (x[0], x[0], x[1], x[2])):
+            assert u.shape == w.shape and bool((u == 0).all())
+
+
+@gpu
+def test_captured_and_on_another_stream():
+    q, k, v, do = _inputs("cuda", torch.bfloat16, 2, 150, 150, 4, 2, 64)
+    lens = _t([150, 80], "cuda")
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+
+    def step():
+        out = OF.attention_recompute(*leaves, causal=True, q_lens=lens,
+                                     kv_lens=lens)
+        grads = torch.autograd.grad(out, leaves, do)
+        return [x.detach() for x in (out, *grads)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(first, step()):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        with torch.no_grad():
+            for x in leaves:
+                x.copy_(torch.randn_like(x, dtype=torch.float32))
+            lens.copy_(torch.tensor([150 - 40 * i, 10 * i]))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_refusals(dev):
+    def z(*s, dt=torch.bfloat16):
+        return torch.zeros(*s, device=dev, dtype=dt)
+
+    q, k = z(2, 4, 6, 64), z(2, 5, 2, 64)
+    for a, kw in (
+            ((q[0], k[0], k[0]), {}),
+            ((q, k, z(2, 6, 2, 64)), {}),
+            ((q, z(1, 5, 2, 64), z(1, 5, 2, 64)), {}),
+            ((q, z(2, 5, 2, 32), z(2, 5, 2, 32)), {}),
+            ((q, z(2, 5, 4, 64), z(2, 5, 4, 64)), {}),
+            ((q, z(2, 5, 0, 64), z(2, 5, 0, 64)), {}),
+            ((q, k.float(), k.float()), {}),
+            ((q, k, k), {"scale": 0.0}),
+            ((q, k, k), {"scale": -1.0}),
+            ((q, k, k), {"scale": float("nan")}),
+            ((q, k, k), {"kv_lens": z(2)}),
+            ((q, k, k), {"kv_lens": z(3, dt=torch.int32)}),
+            ((q, k, k), {"q_lens": z(2, 1, dt=torch.int32)})):
+        with pytest.raises(ValueError):
+            OF.attention_recompute(*a, **kw)
+
+
+@gpu
+def test_refuses_what_the_kernel_cannot_take():
+    for shape, dt in (((1, 4, 2, 60), torch.bfloat16),
+                      ((1, 4, 2, 136), torch.bfloat16),
+                      ((1, 4, 2, 64), torch.float32)):
+        q = torch.zeros(*shape, device="cuda", dtype=dt)
+        with pytest.raises((ValueError, RuntimeError)):
+            OF.attention_recompute(q, q, q)
+    q = torch.zeros(1, 4, 2, 64, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        OF.attention_recompute(q, q, q, kv_lens=torch.tensor([4]))

@@ -110,12 +110,30 @@ struct Seq {
   }
 };
 
+// Block index -> sequence and head, block of it, and part. Causal: all heads'
+// longest blocks first (LAST: high indexes are long). Else 8 heads at a time.
+// Either way a head's blocks are 8 (or bh) apart, and as the hardware deals
+// blocks out to its 8 dies in turn, they meet in one die's L2.
+DEV_INLINE void place(const Args& a, int nblk, bool last, int* bh, int* blk) {
+  int heads = a.b * a.hk, i = blockIdx.x;
+  if (a.causal) {
+    *blk = i / heads;
+    *bh = i - *blk * heads;
+    if (last) *blk = nblk - 1 - *blk;
+  } else {
+    int grp = i / (8 * nblk), w = i - grp * 8 * nblk;
+    int n = heads - grp * 8;
+    n = n < 8 ? n : 8;
+    *blk = w / n;
+    *bh = grp * 8 + w - *blk * n;
+  }
+}
+
 template <int HDT> struct Geo {
   static constexpr int NCH = HDT == 64 ? 8 : 16;  // chunks of an LDS row
   static constexpr int PITCH = NCH * 16;
   static constexpr int KS = HDT / 16;  // k steps of a product over the head
   static constexpr int DT = HDT / 32;  // 32-column tiles of the head
-  static constexpr int BYTES = TILE * PITCH;
 };
 
 DEV_INLINE int perm(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
@@ -156,15 +174,16 @@ DEV_INLINE void to_lds4(const void* src, void* dst) {
   __builtin_amdgcn_global_load_lds((gp_t)src, (lp_t)dst, 4, 0, 0);
 }
 
-// Tile of 64 rows r0.. below `end` to LDS, by NW waves. PACKED: row r is
+// Tile of R rows r0.. below `end` to LDS, by 4 waves. PACKED: row r is
 // position r / g of head r % g, else position r.
-template <int HDT, int NW, bool PACKED>
+template <int HDT, int R, bool PACKED>
 DEV_INLINE void stage(const Args& a, const char* base, long ss, long sh,
                       int r0, int end, char* lds, int wave, int lane) {
-  constexpr int NCH = Geo<HDT>::NCH, RPI = 64 / NCH;
+  constexpr int NCH = Geo<HDT>::NCH, RPI = 64 / NCH, N = R / RPI / 4;
+  static_assert(N > 0, "a wave stages at least one piece");
 #pragma unroll
-  for (int i = 0; i < TILE / RPI / NW; ++i) {
-    int idx = wave * (TILE / RPI / NW) + i;
+  for (int i = 0; i < N; ++i) {
+    int idx = wave * N + i;
     int row = idx * RPI + lane / NCH;
     int chunk = (lane % NCH) ^ perm(row);
     int r = r0 + row;
@@ -260,11 +279,11 @@ struct Row {
 template <typename T, int HDT>
 __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk) {
   using G = Geo<HDT>;
-  __shared__ __attribute__((aligned(16))) char ktile[2][G::BYTES];
-  __shared__ __attribute__((aligned(16))) char vtile[2][G::BYTES];
+  __shared__ __attribute__((aligned(16))) char ktile[2][TILE * G::PITCH];
+  __shared__ __attribute__((aligned(16))) char vtile[2][TILE * G::PITCH];
   int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  int bh = blockIdx.x / nblk;
-  int blk = nblk - 1 - (blockIdx.x - bh * nblk);  // longest rows first
+  int bh, blk;
+  place(a, nblk, true, &bh, &blk);
   Seq s(a, bh);
   Row row(a, s, blk * 128 + wave * 32 + (lane & 31));
   const char* kb = reinterpret_cast<const char*>(a.k.p) +
@@ -291,15 +310,15 @@ __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk) {
   for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
 
   if (ntile) {
-    stage<HDT, 4, false>(a, kb, a.k.ss, 0, 0, s.klen, ktile[0], wave, lane);
-    stage<HDT, 4, false>(a, vb, a.v.ss, 0, 0, s.klen, vtile[0], wave, lane);
+    stage<HDT, TILE, false>(a, kb, a.k.ss, 0, 0, s.klen, ktile[0], wave, lane);
+    stage<HDT, TILE, false>(a, vb, a.v.ss, 0, 0, s.klen, vtile[0], wave, lane);
   }
   staged();
   for (int t = 0; t < ntile; ++t) {
     if (t + 1 < ntile) {
-      stage<HDT, 4, false>(a, kb, a.k.ss, 0, (t + 1) * TILE, s.klen,
+      stage<HDT, TILE, false>(a, kb, a.k.ss, 0, (t + 1) * TILE, s.klen,
                            ktile[(t + 1) & 1], wave, lane);
-      stage<HDT, 4, false>(a, vb, a.v.ss, 0, (t + 1) * TILE, s.klen,
+      stage<HDT, TILE, false>(a, vb, a.v.ss, 0, (t + 1) * TILE, s.klen,
                            vtile[(t + 1) & 1], wave, lane);
     }
     const char *kt = ktile[t & 1], *vt = vtile[t & 1];
@@ -377,11 +396,11 @@ __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk) {
 template <typename T, int HDT>
 __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk) {
   using G = Geo<HDT>;
-  __shared__ __attribute__((aligned(16))) char ktile[2][G::BYTES];
-  __shared__ __attribute__((aligned(16))) char vtile[2][G::BYTES];
+  __shared__ __attribute__((aligned(16))) char ktile[2][TILE * G::PITCH];
+  __shared__ __attribute__((aligned(16))) char vtile[2][TILE * G::PITCH];
   int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  int bh = blockIdx.x / nblk;
-  int blk = nblk - 1 - (blockIdx.x - bh * nblk);
+  int bh, blk;
+  place(a, nblk, true, &bh, &blk);
   Seq s(a, bh);
   Row row(a, s, blk * 128 + wave * 32 + (lane & 31));
   const char* kb = reinterpret_cast<const char*>(a.k.p) +
@@ -395,8 +414,8 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk) {
   int ntile = end > 0 ? (end + TILE - 1) / TILE : 0;
   int wlo = wave_min(row.lim), whi = wave_max(row.valid ? row.lim : 0);
   if (ntile) {
-    stage<HDT, 4, false>(a, kb, a.k.ss, 0, 0, s.klen, ktile[0], wave, lane);
-    stage<HDT, 4, false>(a, vb, a.v.ss, 0, 0, s.klen, vtile[0], wave, lane);
+    stage<HDT, TILE, false>(a, kb, a.k.ss, 0, 0, s.klen, ktile[0], wave, lane);
+    stage<HDT, TILE, false>(a, vb, a.v.ss, 0, 0, s.klen, vtile[0], wave, lane);
   }
   s16x8 qf[G::KS], df[G::KS];
   keep<HDT>(a,
@@ -436,16 +455,16 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk) {
   staged();
   for (int t = 0; t < ntile; ++t) {
     if (t + 1 < ntile) {
-      stage<HDT, 4, false>(a, kb, a.k.ss, 0, (t + 1) * TILE, s.klen,
+      stage<HDT, TILE, false>(a, kb, a.k.ss, 0, (t + 1) * TILE, s.klen,
                            ktile[(t + 1) & 1], wave, lane);
-      stage<HDT, 4, false>(a, vb, a.v.ss, 0, (t + 1) * TILE, s.klen,
+      stage<HDT, TILE, false>(a, vb, a.v.ss, 0, (t + 1) * TILE, s.klen,
                            vtile[(t + 1) & 1], wave, lane);
     }
     const char *kt = ktile[t & 1], *vt = vtile[t & 1];
     int k0 = t * TILE;
-    if (k0 < whi)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
+        if (k0 + u * 32 >= whi) continue;
         f32x16 sc = kNone, dp = kNone;
 #pragma unroll
         for (int ks = 0; ks < G::KS; ++ks)
@@ -487,31 +506,39 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk) {
 }
 
 // ---- backward 2: dK, dV of 128 keys, over all packed rows -----------------
+// Kept in registers: the wave's 32 keys' K, and dK, dV (64 each at a head of
+// 128). V as well would spill there, so from heads of 96 on it stays in LDS
+// and rows stream 32 at a time to leave room for two blocks a CU.
+// With few key blocks the rows are dealt out to `nsplit` blocks in turn
+// (tile t to block t % nsplit), whose fp32 sums a last kernel adds.
 template <typename T, int HDT>
-__global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk) {
+__global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
+                                                        int nsplit,
+                                                        float* part) {
   using G = Geo<HDT>;
-  __shared__ __attribute__((aligned(16))) char qtile[2][G::BYTES];
-  __shared__ __attribute__((aligned(16))) char dtile[2][G::BYTES];
-  __shared__ __attribute__((aligned(16))) float stat[2][2][TILE];
+  constexpr bool VLDS = HDT > 64;
+  constexpr int RT = VLDS ? 32 : 64;
+  __shared__ __attribute__((aligned(16))) char qtile[2][RT * G::PITCH];
+  __shared__ __attribute__((aligned(16))) char dtile[2][RT * G::PITCH];
+  __shared__ __attribute__((aligned(16))) char vkeep[VLDS ? 128 * G::PITCH
+                                                          : 16];
+  __shared__ __attribute__((aligned(16))) float stat[2][2][64];
   int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  int bh = blockIdx.x / nblk;
-  int blk = blockIdx.x - bh * nblk;  // the first keys are seen most
+  int bh, blk;
+  place(a, nblk * nsplit, false, &bh, &blk);
+  int split = blk % nsplit;
+  blk /= nsplit;
   Seq s(a, bh);
   int key = blk * 128 + wave * 32 + (lane & 31);
   bool valid = key < s.klen;
-  s16x8 kf[G::KS], vf[G::KS];
-  keep<HDT>(a,
-            reinterpret_cast<const char*>(a.k.p) +
-                2 * (s.batch * a.k.sb + s.kvh * a.k.sh + key * a.k.ss),
-            valid, lane, kf);
-  keep<HDT>(a,
-            reinterpret_cast<const char*>(a.v.p) +
-                2 * (s.batch * a.v.sb + s.kvh * a.v.sh + key * a.v.ss),
-            valid, lane, vf);
   const char* qb = reinterpret_cast<const char*>(a.q.p) +
                    2 * (s.batch * a.q.sb + (long)s.kvh * a.g * a.q.sh);
   const char* db = reinterpret_cast<const char*>(a.dout.p) +
                    2 * (s.batch * a.dout.sb + (long)s.kvh * a.g * a.dout.sh);
+  const char* kb = reinterpret_cast<const char*>(a.k.p) +
+                   2 * (s.batch * a.k.sb + s.kvh * a.k.sh);
+  const char* vb = reinterpret_cast<const char*>(a.v.p) +
+                   2 * (s.batch * a.v.sb + s.kvh * a.v.sh);
   const float* lse = a.lse + (long)bh * a.sq * a.g;
   const float* del = a.delta + (long)bh * a.sq * a.g;
   // rows from `lo` on see this lane's key
@@ -519,19 +546,19 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk) {
   if (a.causal) lo = key > s.off ? (key - s.off) * a.g : 0;
   int first = 0;
   if (a.causal && blk * 128 > s.off) first = (blk * 128 - s.off) * a.g;
-  first &= ~(TILE - 1);
+  first &= ~(RT - 1);
   int ntile = 0;
   if (blk * 128 < s.klen && first < s.rows)
-    ntile = (s.rows - first + TILE - 1) / TILE;
+    ntile = (s.rows - first + RT - 1) / RT;
   int wlo = wave_min(lo), whi = wave_max(valid ? lo : 0);
   bool wlive = wave_max(valid) != 0;
 
-  auto load = [&](int t) {
-    int r0 = first + t * TILE, buf = t & 1;
-    stage<HDT, 4, true>(a, qb, a.q.ss, a.q.sh, r0, s.rows, qtile[buf], wave,
-                        lane);
-    stage<HDT, 4, true>(a, db, a.dout.ss, a.dout.sh, r0, s.rows, dtile[buf],
-                        wave, lane);
+  auto load = [&](int t, int buf) {
+    int r0 = first + t * RT;
+    stage<HDT, RT, true>(a, qb, a.q.ss, a.q.sh, r0, s.rows, qtile[buf], wave,
+                         lane);
+    stage<HDT, RT, true>(a, db, a.dout.ss, a.dout.sh, r0, s.rows, dtile[buf],
+                         wave, lane);
     if (wave < 2) {
       bool in = r0 + lane < s.rows;
       const float* src = wave ? (in ? del + r0 + lane
@@ -540,63 +567,75 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk) {
       to_lds4(src, stat[buf][wave]);
     }
   };
+  s16x8 kf[G::KS], vf[VLDS ? 1 : G::KS];
+  if (split < ntile) {
+    load(split, 0);
+    if (VLDS)
+      stage<HDT, 128, false>(a, vb, a.v.ss, 0, blk * 128, s.klen, vkeep, wave,
+                             lane);
+  }
+  keep<HDT>(a, kb + 2 * (key * a.k.ss), valid, lane, kf);
+  if (!VLDS) keep<HDT>(a, vb + 2 * (key * a.v.ss), valid, lane, vf);
   float c = a.scale * kLog2e;
   f32x16 dk[G::DT], dv[G::DT];
 #pragma unroll
   for (int i = 0; i < G::DT; ++i) dk[i] = dv[i] = kNone;
-  if (ntile) load(0);
   staged();
-  for (int t = 0; t < ntile; ++t) {
-    if (t + 1 < ntile) load(t + 1);
-    const char *qt = qtile[t & 1], *dt = dtile[t & 1];
-    const float *ls = stat[t & 1][0], *ds = stat[t & 1][1];
-    int r0 = first + t * TILE;
-    if (wlive && r0 + TILE > wlo)
+  int buf = 0;
+  for (int t = split; t < ntile; t += nsplit, buf ^= 1) {
+    if (t + nsplit < ntile) load(t + nsplit, buf ^ 1);
+    const char *qt = qtile[buf], *dt = dtile[buf];
+    const float *ls = stat[buf][0], *ds = stat[buf][1];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        f32x16 sc = kNone, dp = kNone;
+    for (int u = 0; u < RT / 32; ++u) {
+      int r0 = first + t * RT + u * 32;
+      if (!wlive || r0 + 32 <= wlo || r0 >= s.rows) continue;
+      f32x16 sc = kNone, dp = kNone;
 #pragma unroll
-        for (int ks = 0; ks < G::KS; ++ks)
-          sc = Op<T>::mfma(frag_row<HDT>(qt, u * 32, ks, lane), kf[ks], sc);
+      for (int ks = 0; ks < G::KS; ++ks)
+        sc = Op<T>::mfma(frag_row<HDT>(qt, u * 32, ks, lane), kf[ks], sc);
 #pragma unroll
-        for (int ks = 0; ks < G::KS; ++ks)
-          dp = Op<T>::mfma(frag_row<HDT>(dt, u * 32, ks, lane), vf[ks], dp);
-        if (r0 + u * 32 < whi)
+      for (int ks = 0; ks < G::KS; ++ks)
+        dp = Op<T>::mfma(frag_row<HDT>(dt, u * 32, ks, lane),
+                         VLDS ? frag_row<HDT>(vkeep, wave * 32, ks, lane)
+                              : vf[VLDS ? 0 : ks],
+                         dp);
+      if (r0 < whi)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            int r = r0 + u * 32 + (i >> 2) * 8 + h * 4 + (i & 3);
-            sc[i] = r >= lo ? sc[i] : -INFINITY;
-          }
-        unsigned p[8], d[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float4 l4 = *reinterpret_cast<const float4*>(ls + u * 32 + j * 8 +
-                                                       h * 4);
-          float4 d4 = *reinterpret_cast<const float4*>(ds + u * 32 + j * 8 +
-                                                       h * 4);
-          const float *lp = &l4.x, *dl = &d4.x;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float x = __builtin_amdgcn_exp2f(
-                fmaf(sc[4 * j + 2 * i], c, -lp[2 * i]));
-            float y = __builtin_amdgcn_exp2f(
-                fmaf(sc[4 * j + 2 * i + 1], c, -lp[2 * i + 1]));
-            p[2 * j + i] = Op<T>::pack(x, y);
-            d[2 * j + i] = Op<T>::pack(x * (dp[4 * j + 2 * i] - dl[2 * i]),
-                                       y * (dp[4 * j + 2 * i + 1] -
-                                            dl[2 * i + 1]));
-          }
+        for (int i = 0; i < 16; ++i) {
+          int r = r0 + (i >> 2) * 8 + h * 4 + (i & 3);
+          sc[i] = r >= lo ? sc[i] : -INFINITY;
         }
+      unsigned p[8], d[8];
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+      for (int j = 0; j < 4; ++j) {
+        float4 l4 =
+            *reinterpret_cast<const float4*>(ls + u * 32 + j * 8 + h * 4);
+        float4 d4 =
+            *reinterpret_cast<const float4*>(ds + u * 32 + j * 8 + h * 4);
+        const float *lp = &l4.x, *dl = &d4.x;
 #pragma unroll
-          for (int i = 0; i < G::DT; ++i) {
-            dv[i] = Op<T>::mfma(frag_col<HDT>(dt, u * 32 + k * 16, i, lane),
-                                pack8(p + 4 * k), dv[i]);
-            dk[i] = Op<T>::mfma(frag_col<HDT>(qt, u * 32 + k * 16, i, lane),
-                                pack8(d + 4 * k), dk[i]);
-          }
+        for (int i = 0; i < 2; ++i) {
+          float x = __builtin_amdgcn_exp2f(
+              fmaf(sc[4 * j + 2 * i], c, -lp[2 * i]));
+          float y = __builtin_amdgcn_exp2f(
+              fmaf(sc[4 * j + 2 * i + 1], c, -lp[2 * i + 1]));
+          p[2 * j + i] = Op<T>::pack(x, y);
+          d[2 * j + i] =
+              Op<T>::pack(x * (dp[4 * j + 2 * i] - dl[2 * i]),
+                          y * (dp[4 * j + 2 * i + 1] - dl[2 * i + 1]));
+        }
       }
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < G::DT; ++i) {
+          dv[i] = Op<T>::mfma(frag_col<HDT>(dt, u * 32 + k * 16, i, lane),
+                              pack8(p + 4 * k), dv[i]);
+          dk[i] = Op<T>::mfma(frag_col<HDT>(qt, u * 32 + k * 16, i, lane),
+                              pack8(d + 4 * k), dk[i]);
+        }
+    }
     staged();
   }
   if (key >= a.sk) return;
@@ -604,12 +643,62 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk) {
 #pragma unroll
     for (int i = 0; i < G::DT; ++i) dk[i] = dv[i] = kNone;
   long at = (((long)s.batch * a.sk + key) * a.hk + s.kvh) * a.hd;
-  put_row<T, G::DT>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, a.hd, lane);
-  put_row<T, G::DT>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, a.hd, lane);
+  if (nsplit == 1) {
+    put_row<T, G::DT>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, a.hd, lane);
+    put_row<T, G::DT>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, a.hd,
+                      lane);
+    return;
+  }
+  long n = (long)a.b * a.sk * a.hk * a.hd;
+  float* out = part + 2 * split * n + at;
+#pragma unroll
+  for (int i = 0; i < G::DT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      int e = i * 32 + j * 8 + h * 4;
+      if (e < a.hd) {
+        *reinterpret_cast<float4*>(out + e) = {dk[i][4 * j], dk[i][4 * j + 1],
+                                               dk[i][4 * j + 2],
+                                               dk[i][4 * j + 3]};
+        *reinterpret_cast<float4*>(out + n + e) = {
+            dv[i][4 * j], dv[i][4 * j + 1], dv[i][4 * j + 2],
+            dv[i][4 * j + 3]};
+      }
+    }
+}
+
+// dk, dv = sums over the splits' part[split][2][n], 4 elements a thread
+template <typename T>
+__global__ __launch_bounds__(256) void attn_rc_join_k(
+    const float* __restrict__ part, long n, int nsplit, float scale,
+    T* __restrict__ dk, T* __restrict__ dv) {
+  long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= 2 * n) return;
+  float4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < nsplit; ++k) {
+    float4 x = *reinterpret_cast<const float4*>(part + 2 * k * n + i);
+    sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+  }
+  float m = i < n ? scale : 1.f;
+  uint2 v = {Op<T>::pack(sum.x * m, sum.y * m),
+             Op<T>::pack(sum.z * m, sum.w * m)};
+  *reinterpret_cast<uint2*>(i < n ? dk + i : dv + (i - n)) = v;
+}
+
+// Blocks that share a key block's rows. Two blocks run on each of 256 CUs;
+// below four rounds of them (a causal mask's blocks differ in length) rows
+// are dealt out, 512 at least to each.
+int dkv_splits(long b, long sq, long sk, long hk, long g) {
+  long blocks = b * hk * ((sk + 127) / 128), rows = sq * g;
+  if (blocks == 0) return 1;
+  long n = (2048 + blocks - 1) / blocks;
+  if (n > rows / 512) n = rows / 512;
+  if (n > 16) n = 16;
+  return n < 1 ? 1 : (int)n;
 }
 
 template <typename T, int HDT>
-void launch(const Args& a, int bwd, hipStream_t s) {
+void launch(const Args& a, int bwd, float* part, hipStream_t s) {
   int rblk = (a.sq * a.g + 127) / 128, kblk = (a.sk + 127) / 128;
   int bh = a.b * a.hk;
   if (!bwd) {
@@ -617,24 +706,39 @@ void launch(const Args& a, int bwd, hipStream_t s) {
     return;
   }
   if (rblk) attn_rc_dq_k<T, HDT><<<bh * rblk, 256, 0, s>>>(a, rblk);
-  if (kblk) attn_rc_dkv_k<T, HDT><<<bh * kblk, 256, 0, s>>>(a, kblk);
+  if (!kblk) return;
+  int nsplit = dkv_splits(a.b, a.sq, a.sk, a.hk, a.g);
+  attn_rc_dkv_k<T, HDT><<<bh * kblk * nsplit, 256, 0, s>>>(a, kblk, nsplit,
+                                                           part);
+  if (nsplit > 1) {
+    long n = (long)a.b * a.sk * a.hk * a.hd;
+    attn_rc_join_k<T><<<(n / 2 + 255) / 256, 256, 0, s>>>(
+        part, n, nsplit, a.scale, (T*)a.dk, (T*)a.dv);
+  }
 }
 
 }  // namespace
 
 extern "C" {
 
+// floats of workspace that backward needs
+long pdta_attn_recompute_ws(long b, long sq, long sk, long hk, long g,
+                            long hd) {
+  int n = dkv_splits(b, sq, sk, hk, g);
+  return n > 1 ? 2 * n * b * sk * hk * hd : 0;
+}
+
 // strides: q, k, v, dout, each (b, s, head) in elements; multiples of 8, all
 // pointers 16-byte aligned, hd a multiple of 8 up to 128. lens null or [b].
 // Forward writes out and, unless null, lse; backward reads both and writes
-// delta, dq, dk, dv. Grids must stay below 2^31 blocks and sq*g below 2^31.
+// delta, dq, dk, dv, with pdta_attn_recompute_ws floats in ws. Grids must stay below 2^31 blocks and sq*g below 2^31.
 void pdta_attn_recompute(const void* q, const void* k, const void* v,
                          const void* dout, const long* st, void* out,
                          float* lse, float* delta, void* dq, void* dk,
                          void* dv, const void* q_lens, const void* kv_lens,
                          int lens64, int b, int sq, int sk, int hk, int g,
-                         int hd, float scale, int causal, int bwd, int dt,
-                         hipStream_t s) {
+                         int hd, float scale, int causal, int bwd,
+                         float* ws, int dt, hipStream_t s) {
   Args a;
   a.q = {q, st[0], st[1], st[2]};
   a.k = {k, st[3], st[4], st[5]};
@@ -649,11 +753,11 @@ void pdta_attn_recompute(const void* q, const void* k, const void* v,
   if (b == 0 || hk == 0) return;
   PDTA_DISPATCH_DTYPE16(dt, T, {
     if (hd <= 64)
-      launch<T, 64>(a, bwd, s);
+      launch<T, 64>(a, bwd, ws, s);
     else if (hd <= 96)
-      launch<T, 96>(a, bwd, s);
+      launch<T, 96>(a, bwd, ws, s);
     else
-      launch<T, 128>(a, bwd, s);
+      launch<T, 128>(a, bwd, ws, s);
   });
 }
 

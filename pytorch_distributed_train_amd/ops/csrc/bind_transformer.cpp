@@ -23,7 +23,9 @@ void pdta_qknorm(const void* const*, const long*, const void* const*,
 void pdta_attn_recompute(const void*, const void*, const void*, const void*,
                          const long*, void*, float*, float*, void*, void*,
                          void*, const void*, const void*, int, int, int, int,
-                         int, int, int, float, int, int, int, hipStream_t);
+                         int, int, int, float, int, int, float*, int,
+                         hipStream_t);
+long pdta_attn_recompute_ws(long, long, long, long, long, long);
 }
 
 namespace {
@@ -274,7 +276,8 @@ AttnShape attn_check(const at::Tensor& q, const at::Tensor& k,
   }
   long g = n.hk ? n.h / n.hk : 1;
   TORCH_CHECK((n.sq + n.sk + 1024) * g < (1l << 31) &&
-                  n.b * n.hk * ((n.sq * g + n.sk) / 128 + 2) < (1l << 31),
+                  n.b * n.hk * ((n.sq * g + n.sk) / 128 + 2) * 16 <
+                      (1l << 31),
               "attention: too many rows");
   for (const auto* l : {&q_lens, &kv_lens})
     if (l->has_value()) {
@@ -333,7 +336,7 @@ std::vector<at::Tensor> attn_recompute_fwd(
                         nullptr, nullptr, nullptr, len_ptr(q_lens),
                         len_ptr(kv_lens), lens_wide(q_lens, kv_lens), n.b,
                         n.sq, n.sk, n.hk, g, n.hd, (float)scale, causal, 0,
-                        dt_of(q), cur_stream());
+                        nullptr, dt_of(q), cur_stream());
     launched("attn_recompute_fwd");
   }
   return {out, lse};
@@ -364,6 +367,9 @@ std::vector<at::Tensor> attn_recompute_bwd(
   auto dk = at::empty({n.b, n.sk, n.hk, n.hd}, q.options());
   auto dv = at::empty_like(dk);
   auto delta = at::empty_like(lse);
+  auto ws = at::empty(
+      {pdta_attn_recompute_ws(n.b, n.sq, n.sk, n.hk, g, n.hd)},
+      lse.options());
   long st[12];
   attn_strides(q, st);
   attn_strides(k, st + 3);
@@ -376,8 +382,8 @@ std::vector<at::Tensor> attn_recompute_bwd(
                         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                         len_ptr(q_lens), len_ptr(kv_lens),
                         lens_wide(q_lens, kv_lens), n.b, n.sq, n.sk, n.hk, g,
-                        n.hd, (float)scale, causal, 1, dt_of(q),
-                        cur_stream());
+                        n.hd, (float)scale, causal, 1, ws.data_ptr<float>(),
+                        dt_of(q), cur_stream());
     launched("attn_recompute_bwd");
   }
   return {dq, dk, dv};

@@ -72,6 +72,7 @@ template <> struct Op<__half> {
 struct View {  // [b, s, heads, hd] of a 16-bit type, strides in elements
   const void* p;
   long sb, ss, sh;
+  bool quick;  // see Stream
 };
 
 struct Args {
@@ -164,42 +165,108 @@ DEV_INLINE s16x8 frag_col(const char* lds, int r0, int dt, int lane) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-typedef const __attribute__((address_space(1))) uint32_t* gp_t;
-typedef __attribute__((address_space(3))) uint32_t* lp_t;
-// global to LDS: lane l's 16 (4) bytes land at dst + 16 (4) * l
+// Global to LDS: lane l's 16 (4) bytes land at dst + 16 (4) * l. In assembly
+// and not by the builtin, since the compiler would make LDS reads of the other
+// buffer wait for these loads; staged() waits for them. They have no output
+// register, and an uncounted load in flight only makes the compiler's own
+// waits longer.
+DEV_INLINE unsigned lds_base(const void* p) {
+  return __builtin_amdgcn_readfirstlane(
+      (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
+}
 DEV_INLINE void to_lds16(const void* src, void* dst) {
-  __builtin_amdgcn_global_load_lds((gp_t)src, (lp_t)dst, 16, 0, 0);
+  asm volatile(
+      "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+      :
+      : "v"(src), "s"(lds_base(dst))
+      : "memory", "m0");
+}
+// from the wave's `base` plus the lane's 32-bit offset
+DEV_INLINE void to_lds16(const void* base, unsigned off, void* dst) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+      :
+      : "v"(off), "s"(base), "s"(lds_base(dst))
+      : "memory", "m0");
 }
 DEV_INLINE void to_lds4(const void* src, void* dst) {
-  __builtin_amdgcn_global_load_lds((gp_t)src, (lp_t)dst, 4, 0, 0);
+  asm volatile(
+      "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
+      :
+      : "v"(src), "s"(lds_base(dst))
+      : "memory", "m0");
 }
 
-// Tile of R rows r0.. below `end` to LDS, by 4 waves. PACKED: row r is
-// position r / g of head r % g, else position r.
+// A streamed operand: rows r0.. below `end` of one sequence and head go to
+// LDS in tiles of R rows, by 4 waves. PACKED: row r is position r / g of head
+// r % g, else position r. A wave's load moves RPI = 4 or 8 rows. In a whole
+// tile their addresses are a scalar base and a lane's offset that never
+// changes (`quick`: RPI rows must not straddle positions unevenly, so g
+// divides RPI or RPI g); lanes past the head's end fetch its first chunk,
+// whose partner in the product is 0 or whose result is not stored. The last
+// tile works out each lane's row and fetches zeros beyond the end.
 template <int HDT, int R, bool PACKED>
-DEV_INLINE void stage(const Args& a, const char* base, long ss, long sh,
-                      int r0, int end, char* lds, int wave, int lane) {
-  constexpr int NCH = Geo<HDT>::NCH, RPI = 64 / NCH, N = R / RPI / 4;
-  static_assert(N > 0, "a wave stages at least one piece");
+struct Stream {
+  static constexpr int NCH = Geo<HDT>::NCH, RPI = 64 / NCH, N = R / RPI / 4;
+  static_assert(N > 0 && (NCH == 8 || N % 2 == 0), "pieces a wave");
+  const char* base;
+  long ss, sh;
+  unsigned off[2];  // even and odd pieces (their rows' perm differs)
+  bool quick;
+
+  DEV_INLINE Stream(const Args& a, const View& v, const Seq& s, int lane) {
+    ss = v.ss, sh = v.sh;
+    base = reinterpret_cast<const char*>(v.p) +
+           2 * (s.batch * v.sb + (long)s.kvh * (PACKED ? a.g : 1) * sh);
+    quick = v.quick;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    int idx = wave * N + i;
-    int row = idx * RPI + lane / NCH;
-    int chunk = (lane % NCH) ^ perm(row);
-    int r = r0 + row;
-    long at;
-    if (PACKED) {
-      int pos = (int)mdiv(r, a.g_mul, a.g_shift);
-      at = pos * ss + (r - pos * a.g) * sh;
-    } else {
-      at = r * ss;
+    for (int k = 0; k < 2; ++k) {
+      int l = lane / NCH;
+      int chunk = (lane % NCH) ^ perm(NCH == 8 ? l : l + 4 * k);
+      if (chunk * 8 >= a.hd) chunk = 0;
+      long at = PACKED ? (l / a.g) * ss + (l % a.g) * sh : l * ss;
+      off[k] = (unsigned)(2 * at) + chunk * 16;
     }
-    const char* src = base + 2 * (at + chunk * 8);
-    if (r >= end || chunk * 8 >= a.hd)
-      src = reinterpret_cast<const char*>(&kZeros);
-    to_lds16(src, lds + idx * 1024);
   }
-}
+
+  DEV_INLINE void load(const Args& a, int r0, int end, char* lds, int wave,
+                       int lane) const {
+    if (quick && r0 + R <= end) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        int idx = wave * N + i, x = r0 + idx * RPI;
+        long at;
+        if (PACKED) {
+          int pos = (int)mdiv(x, a.g_mul, a.g_shift);
+          at = pos * ss + (x - pos * a.g) * sh;
+        } else {
+          at = x * ss;
+        }
+        to_lds16(base + 2 * at, off[NCH == 8 ? 0 : i & 1], lds + idx * 1024);
+      }
+      return;
+    }
+    asm volatile("" : "+v"(lane));  // keeps this out of the loop's registers
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      int idx = wave * N + i;
+      int row = idx * RPI + lane / NCH;
+      int chunk = (lane % NCH) ^ perm(row);
+      int r = r0 + row;
+      long at;
+      if (PACKED) {
+        int pos = (int)mdiv(r, a.g_mul, a.g_shift);
+        at = pos * ss + (r - pos * a.g) * sh;
+      } else {
+        at = r * ss;
+      }
+      const char* src = base + 2 * at + chunk * 16;
+      if (r >= end || chunk * 8 >= a.hd)
+        src = reinterpret_cast<const char*>(&kZeros);
+      to_lds16(src, lds + idx * 1024);
+    }
+  }
+};
 
 // the lane's row of a kept operand, in registers
 template <int HDT>
@@ -240,6 +307,13 @@ DEV_INLINE s16x8 pack8(const unsigned* p) {
   return __builtin_bit_cast(s16x8, v);
 }
 
+// Buffers are arrays of their own and steps come in pairs that name them: a
+// read of one buffer then provably does not wait for the loads in flight to
+// the other (as one array indexed by step & 1, every step waited for the next
+// one's loads).
+#define LDS_BUFFER(name, bytes) \
+  __shared__ __attribute__((aligned(16))) char name[bytes]
+
 DEV_INLINE void staged() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
@@ -279,17 +353,17 @@ struct Row {
 template <typename T, int HDT>
 __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk) {
   using G = Geo<HDT>;
-  __shared__ __attribute__((aligned(16))) char ktile[2][TILE * G::PITCH];
-  __shared__ __attribute__((aligned(16))) char vtile[2][TILE * G::PITCH];
-  int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  LDS_BUFFER(k0, TILE * G::PITCH);
+  LDS_BUFFER(k1, TILE * G::PITCH);
+  LDS_BUFFER(v0, TILE * G::PITCH);
+  LDS_BUFFER(v1, TILE * G::PITCH);
+  int lane = threadIdx.x & 63, h = lane >> 5;
+  int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int bh, blk;
   place(a, nblk, true, &bh, &blk);
   Seq s(a, bh);
   Row row(a, s, blk * 128 + wave * 32 + (lane & 31));
-  const char* kb = reinterpret_cast<const char*>(a.k.p) +
-                   2 * (s.batch * a.k.sb + s.kvh * a.k.sh);
-  const char* vb = reinterpret_cast<const char*>(a.v.p) +
-                   2 * (s.batch * a.v.sb + s.kvh * a.v.sh);
+  Stream<HDT, TILE, false> kin(a, a.k, s, lane), vin(a, a.v, s, lane);
   s16x8 qf[G::KS];
   keep<HDT>(a,
             reinterpret_cast<const char*>(a.q.p) +
@@ -309,73 +383,70 @@ __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk) {
 #pragma unroll
   for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
 
-  if (ntile) {
-    stage<HDT, TILE, false>(a, kb, a.k.ss, 0, 0, s.klen, ktile[0], wave, lane);
-    stage<HDT, TILE, false>(a, vb, a.v.ss, 0, 0, s.klen, vtile[0], wave, lane);
-  }
+  auto load = [&](int t, char* kd, char* vd) {
+    kin.load(a, t * TILE, s.klen, kd, wave, lane);
+    vin.load(a, t * TILE, s.klen, vd, wave, lane);
+  };
+  auto step = [&](int t, const char* kt, const char* vt) {
+    int key0 = t * TILE;
+    if (key0 >= whi) return;
+    f32x16 sc[2] = {kNone, kNone};
+#pragma unroll
+    for (int ks = 0; ks < G::KS; ++ks)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        sc[u] = Op<T>::mfma(frag_row<HDT>(kt, u * 32, ks, lane), qf[ks],
+                            sc[u]);
+    if (key0 + TILE > wlo) {
+      int rel = row.lim - key0 - h * 4;
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if ((i >> 2) * 8 + (i & 3) >= rel) sc[i >> 4][i & 15] = -INFINITY;
+    }
+    float m = sc[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) m = fmaxf(m, sc[i >> 4][i & 15]);
+    m = fmaxf(m, other_half(m));
+    // P is taken relative to `top`, which follows the running maximum only
+    // when that is 2^8 past it: P stays below 2^8, which neither 16-bit type
+    // minds, and most steps rescale nothing
+    bool up = m > top + far;
+    if (__any(up)) {
+      float f = up ? __builtin_amdgcn_exp2f((top - m) * c) : 1.f;
+      top = up ? m : top;
+      sum *= f;
+#pragma unroll
+      for (int i = 0; i < G::DT; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[i][j] *= f;
+    }
+    float base = top == -INFINITY ? 0.f : -top * c;
+    unsigned p[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float x = __builtin_amdgcn_exp2f(
+          fmaf(sc[i >> 3][(2 * i) & 15], c, base));
+      float y = __builtin_amdgcn_exp2f(
+          fmaf(sc[i >> 3][(2 * i + 1) & 15], c, base));
+      sum += x + y;
+      p[i] = Op<T>::pack(x, y);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < G::DT; ++i)
+        acc[i] = Op<T>::mfma(frag_col<HDT>(vt, k * 16, i, lane),
+                             pack8(p + 4 * k), acc[i]);
+  };
+  if (ntile) load(0, k0, v0);
   staged();
-  for (int t = 0; t < ntile; ++t) {
-    if (t + 1 < ntile) {
-      stage<HDT, TILE, false>(a, kb, a.k.ss, 0, (t + 1) * TILE, s.klen,
-                           ktile[(t + 1) & 1], wave, lane);
-      stage<HDT, TILE, false>(a, vb, a.v.ss, 0, (t + 1) * TILE, s.klen,
-                           vtile[(t + 1) & 1], wave, lane);
-    }
-    const char *kt = ktile[t & 1], *vt = vtile[t & 1];
-    int k0 = t * TILE;
-    if (k0 < whi) {
-      f32x16 sc[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        sc[u] = kNone;
-#pragma unroll
-        for (int ks = 0; ks < G::KS; ++ks)
-          sc[u] = Op<T>::mfma(frag_row<HDT>(kt, u * 32, ks, lane), qf[ks],
-                              sc[u]);
-      }
-      if (k0 + TILE > wlo)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            int key = k0 + u * 32 + (i >> 2) * 8 + h * 4 + (i & 3);
-            sc[u][i] = key < row.lim ? sc[u][i] : -INFINITY;
-          }
-      float m = sc[0][0];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) m = fmaxf(m, sc[i >> 4][i & 15]);
-      m = fmaxf(m, other_half(m));
-      // P is taken relative to `top`, which follows the running maximum
-      // only when that is 2^8 past it: P stays below 2^8, which neither
-      // 16-bit type minds, and most steps rescale nothing
-      bool up = m > top + far;
-      if (__any(up)) {
-        float f = up ? __builtin_amdgcn_exp2f((top - m) * c) : 1.f;
-        top = up ? m : top;
-        sum *= f;
-#pragma unroll
-        for (int i = 0; i < G::DT; ++i)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) acc[i][j] *= f;
-      }
-      float base = top == -INFINITY ? 0.f : -top * c;
-      unsigned p[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float x = __builtin_amdgcn_exp2f(
-            fmaf(sc[i >> 3][(2 * i) & 15], c, base));
-        float y = __builtin_amdgcn_exp2f(
-            fmaf(sc[i >> 3][(2 * i + 1) & 15], c, base));
-        sum += x + y;
-        p[i] = Op<T>::pack(x, y);
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int i = 0; i < G::DT; ++i)
-          acc[i] = Op<T>::mfma(frag_col<HDT>(vt, k * 16, i, lane),
-                               pack8(p + 4 * k), acc[i]);
-    }
+  for (int t = 0; t < ntile; t += 2) {
+    if (t + 1 < ntile) load(t + 1, k1, v1);
+    step(t, k0, v0);
+    staged();
+    if (t + 1 >= ntile) break;
+    if (t + 2 < ntile) load(t + 2, k0, v0);
+    step(t + 1, k1, v1);
     staged();
   }
   sum += other_half(sum);
@@ -396,27 +467,28 @@ __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk) {
 template <typename T, int HDT>
 __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk) {
   using G = Geo<HDT>;
-  __shared__ __attribute__((aligned(16))) char ktile[2][TILE * G::PITCH];
-  __shared__ __attribute__((aligned(16))) char vtile[2][TILE * G::PITCH];
-  int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  LDS_BUFFER(k0, TILE * G::PITCH);
+  LDS_BUFFER(k1, TILE * G::PITCH);
+  LDS_BUFFER(v0, TILE * G::PITCH);
+  LDS_BUFFER(v1, TILE * G::PITCH);
+  int lane = threadIdx.x & 63, h = lane >> 5;
+  int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int bh, blk;
   place(a, nblk, true, &bh, &blk);
   Seq s(a, bh);
   Row row(a, s, blk * 128 + wave * 32 + (lane & 31));
-  const char* kb = reinterpret_cast<const char*>(a.k.p) +
-                   2 * (s.batch * a.k.sb + s.kvh * a.k.sh);
-  const char* vb = reinterpret_cast<const char*>(a.v.p) +
-                   2 * (s.batch * a.v.sb + s.kvh * a.v.sh);
+  Stream<HDT, TILE, false> kin(a, a.k, s, lane), vin(a, a.v, s, lane);
   int last = (blk * 128 + 127) / a.g;
   last = last < s.qlen ? last : s.qlen - 1;
   int end = blk * 128 < s.rows ? s.klen : 0;
   if (a.causal && last + s.off + 1 < end) end = last + s.off + 1;
   int ntile = end > 0 ? (end + TILE - 1) / TILE : 0;
   int wlo = wave_min(row.lim), whi = wave_max(row.valid ? row.lim : 0);
-  if (ntile) {
-    stage<HDT, TILE, false>(a, kb, a.k.ss, 0, 0, s.klen, ktile[0], wave, lane);
-    stage<HDT, TILE, false>(a, vb, a.v.ss, 0, 0, s.klen, vtile[0], wave, lane);
-  }
+  auto load = [&](int t, char* kd, char* vd) {
+    kin.load(a, t * TILE, s.klen, kd, wave, lane);
+    vin.load(a, t * TILE, s.klen, vd, wave, lane);
+  };
+  if (ntile) load(0, k0, v0);
   s16x8 qf[G::KS], df[G::KS];
   keep<HDT>(a,
             reinterpret_cast<const char*>(a.dout.p) +
@@ -452,48 +524,48 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk) {
   f32x16 acc[G::DT];
 #pragma unroll
   for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
-  staged();
-  for (int t = 0; t < ntile; ++t) {
-    if (t + 1 < ntile) {
-      stage<HDT, TILE, false>(a, kb, a.k.ss, 0, (t + 1) * TILE, s.klen,
-                           ktile[(t + 1) & 1], wave, lane);
-      stage<HDT, TILE, false>(a, vb, a.v.ss, 0, (t + 1) * TILE, s.klen,
-                           vtile[(t + 1) & 1], wave, lane);
-    }
-    const char *kt = ktile[t & 1], *vt = vtile[t & 1];
-    int k0 = t * TILE;
+  auto step = [&](int t, const char* kt, const char* vt) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (k0 + u * 32 >= whi) continue;
-        f32x16 sc = kNone, dp = kNone;
+    for (int u = 0; u < 2; ++u) {
+      int key0 = t * TILE + u * 32;
+      if (key0 >= whi) return;
+      f32x16 sc = kNone, dp = kNone;
 #pragma unroll
-        for (int ks = 0; ks < G::KS; ++ks)
-          sc = Op<T>::mfma(frag_row<HDT>(kt, u * 32, ks, lane), qf[ks], sc);
-#pragma unroll
-        for (int ks = 0; ks < G::KS; ++ks)
-          dp = Op<T>::mfma(frag_row<HDT>(vt, u * 32, ks, lane), df[ks], dp);
-        if (k0 + u * 32 + 32 > wlo)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            int key = k0 + u * 32 + (i >> 2) * 8 + h * 4 + (i & 3);
-            sc[i] = key < row.lim ? sc[i] : -INFINITY;
-          }
-        unsigned p[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float x = __builtin_amdgcn_exp2f(fmaf(sc[2 * i], c, -lse)) *
-                    (dp[2 * i] - delta);
-          float y = __builtin_amdgcn_exp2f(fmaf(sc[2 * i + 1], c, -lse)) *
-                    (dp[2 * i + 1] - delta);
-          p[i] = Op<T>::pack(x, y);
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int i = 0; i < G::DT; ++i)
-            acc[i] = Op<T>::mfma(frag_col<HDT>(kt, u * 32 + k * 16, i, lane),
-                                 pack8(p + 4 * k), acc[i]);
+      for (int ks = 0; ks < G::KS; ++ks) {
+        sc = Op<T>::mfma(frag_row<HDT>(kt, u * 32, ks, lane), qf[ks], sc);
+        dp = Op<T>::mfma(frag_row<HDT>(vt, u * 32, ks, lane), df[ks], dp);
       }
+      if (key0 + 32 > wlo) {
+        int rel = row.lim - key0 - h * 4;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if ((i >> 2) * 8 + (i & 3) >= rel) sc[i] = -INFINITY;
+      }
+      unsigned p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float x = __builtin_amdgcn_exp2f(fmaf(sc[2 * i], c, -lse)) *
+                  (dp[2 * i] - delta);
+        float y = __builtin_amdgcn_exp2f(fmaf(sc[2 * i + 1], c, -lse)) *
+                  (dp[2 * i + 1] - delta);
+        p[i] = Op<T>::pack(x, y);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < G::DT; ++i)
+          acc[i] = Op<T>::mfma(frag_col<HDT>(kt, u * 32 + k * 16, i, lane),
+                               pack8(p + 4 * k), acc[i]);
+    }
+  };
+  staged();
+  for (int t = 0; t < ntile; t += 2) {
+    if (t + 1 < ntile) load(t + 1, k1, v1);
+    step(t, k0, v0);
+    staged();
+    if (t + 1 >= ntile) break;
+    if (t + 2 < ntile) load(t + 2, k0, v0);
+    step(t + 1, k1, v1);
     staged();
   }
   if (!row.stored) return;
@@ -518,12 +590,15 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
   using G = Geo<HDT>;
   constexpr bool VLDS = HDT > 64;
   constexpr int RT = VLDS ? 32 : 64;
-  __shared__ __attribute__((aligned(16))) char qtile[2][RT * G::PITCH];
-  __shared__ __attribute__((aligned(16))) char dtile[2][RT * G::PITCH];
-  __shared__ __attribute__((aligned(16))) char vkeep[VLDS ? 128 * G::PITCH
-                                                          : 16];
-  __shared__ __attribute__((aligned(16))) float stat[2][2][64];
-  int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  LDS_BUFFER(q0, RT * G::PITCH);
+  LDS_BUFFER(q1, RT * G::PITCH);
+  LDS_BUFFER(d0, RT * G::PITCH);
+  LDS_BUFFER(d1, RT * G::PITCH);
+  LDS_BUFFER(stat0, 512);  // 64 rows' lse and D
+  LDS_BUFFER(stat1, 512);
+  LDS_BUFFER(vkeep, VLDS ? 128 * G::PITCH : 16);
+  int lane = threadIdx.x & 63, h = lane >> 5;
+  int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int bh, blk;
   place(a, nblk * nsplit, false, &bh, &blk);
   int split = blk % nsplit;
@@ -531,10 +606,7 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
   Seq s(a, bh);
   int key = blk * 128 + wave * 32 + (lane & 31);
   bool valid = key < s.klen;
-  const char* qb = reinterpret_cast<const char*>(a.q.p) +
-                   2 * (s.batch * a.q.sb + (long)s.kvh * a.g * a.q.sh);
-  const char* db = reinterpret_cast<const char*>(a.dout.p) +
-                   2 * (s.batch * a.dout.sb + (long)s.kvh * a.g * a.dout.sh);
+  Stream<HDT, RT, true> qin(a, a.q, s, lane), din(a, a.dout, s, lane);
   const char* kb = reinterpret_cast<const char*>(a.k.p) +
                    2 * (s.batch * a.k.sb + s.kvh * a.k.sh);
   const char* vb = reinterpret_cast<const char*>(a.v.p) +
@@ -553,26 +625,26 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
   int wlo = wave_min(lo), whi = wave_max(valid ? lo : 0);
   bool wlive = wave_max(valid) != 0;
 
-  auto load = [&](int t, int buf) {
+  auto load = [&](int t, char* qd, char* dd, char* sd) {
     int r0 = first + t * RT;
-    stage<HDT, RT, true>(a, qb, a.q.ss, a.q.sh, r0, s.rows, qtile[buf], wave,
-                         lane);
-    stage<HDT, RT, true>(a, db, a.dout.ss, a.dout.sh, r0, s.rows, dtile[buf],
-                         wave, lane);
+    qin.load(a, r0, s.rows, qd, wave, lane);
+    din.load(a, r0, s.rows, dd, wave, lane);
     if (wave < 2) {
       bool in = r0 + lane < s.rows;
       const float* src = wave ? (in ? del + r0 + lane
                                     : reinterpret_cast<const float*>(&kZeros))
                               : (in ? lse + r0 + lane : &kInf);
-      to_lds4(src, stat[buf][wave]);
+      to_lds4(src, sd + wave * 256);
     }
   };
   s16x8 kf[G::KS], vf[VLDS ? 1 : G::KS];
   if (split < ntile) {
-    load(split, 0);
-    if (VLDS)
-      stage<HDT, 128, false>(a, vb, a.v.ss, 0, blk * 128, s.klen, vkeep, wave,
-                             lane);
+    load(split, q0, d0, stat0);
+    if (VLDS) {
+      Stream<HDT, 128, false> vin(a, a.v, s, lane);
+      vin.quick = false;  // zeros past the head's end: dO has none there
+      vin.load(a, blk * 128, s.klen, vkeep, wave, lane);
+    }
   }
   keep<HDT>(a, kb + 2 * (key * a.k.ss), valid, lane, kf);
   if (!VLDS) keep<HDT>(a, vb + 2 * (key * a.v.ss), valid, lane, vf);
@@ -580,32 +652,28 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
   f32x16 dk[G::DT], dv[G::DT];
 #pragma unroll
   for (int i = 0; i < G::DT; ++i) dk[i] = dv[i] = kNone;
-  staged();
-  int buf = 0;
-  for (int t = split; t < ntile; t += nsplit, buf ^= 1) {
-    if (t + nsplit < ntile) load(t + nsplit, buf ^ 1);
-    const char *qt = qtile[buf], *dt = dtile[buf];
-    const float *ls = stat[buf][0], *ds = stat[buf][1];
+  auto step = [&](int t, const char* qt, const char* dt, const char* sd) {
+    const float* ls = reinterpret_cast<const float*>(sd);
+    const float* ds = ls + 64;
 #pragma unroll
     for (int u = 0; u < RT / 32; ++u) {
       int r0 = first + t * RT + u * 32;
       if (!wlive || r0 + 32 <= wlo || r0 >= s.rows) continue;
       f32x16 sc = kNone, dp = kNone;
 #pragma unroll
-      for (int ks = 0; ks < G::KS; ++ks)
+      for (int ks = 0; ks < G::KS; ++ks) {
         sc = Op<T>::mfma(frag_row<HDT>(qt, u * 32, ks, lane), kf[ks], sc);
-#pragma unroll
-      for (int ks = 0; ks < G::KS; ++ks)
         dp = Op<T>::mfma(frag_row<HDT>(dt, u * 32, ks, lane),
                          VLDS ? frag_row<HDT>(vkeep, wave * 32, ks, lane)
                               : vf[VLDS ? 0 : ks],
                          dp);
-      if (r0 < whi)
+      }
+      if (r0 < whi) {
+        int rel = lo - r0 - h * 4;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          int r = r0 + (i >> 2) * 8 + h * 4 + (i & 3);
-          sc[i] = r >= lo ? sc[i] : -INFINITY;
-        }
+        for (int i = 0; i < 16; ++i)
+          if ((i >> 2) * 8 + (i & 3) < rel) sc[i] = -INFINITY;
+      }
       unsigned p[8], d[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -636,6 +704,16 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
                               pack8(d + 4 * k), dk[i]);
         }
     }
+  };
+  staged();
+  for (int t = split; t < ntile; t += 2 * nsplit) {
+    int t1 = t + nsplit, t2 = t1 + nsplit;
+    if (t1 < ntile) load(t1, q1, d1, stat1);
+    step(t, q0, d0, stat0);
+    staged();
+    if (t1 >= ntile) break;
+    if (t2 < ntile) load(t2, q0, d0, stat0);
+    step(t1, q1, d1, stat1);
     staged();
   }
   if (key >= a.sk) return;
@@ -740,10 +818,17 @@ void pdta_attn_recompute(const void* q, const void* k, const void* v,
                          int hd, float scale, int causal, int bwd,
                          float* ws, int dt, hipStream_t s) {
   Args a;
-  a.q = {q, st[0], st[1], st[2]};
-  a.k = {k, st[3], st[4], st[5]};
-  a.v = {v, st[6], st[7], st[8]};
-  a.dout = {dout, st[9], st[10], st[11]};
+  int rpi = hd <= 64 ? 8 : 4;  // rows a load moves
+  bool even = rpi % g == 0 || g % rpi == 0;
+  auto view = [&](const void* x, const long* n, bool packed) {
+    long far = 8 * (n[1] + n[2]) + hd;  // a lane's offset, in elements
+    return View{x, n[0], n[1], n[2],
+                far < (1l << 31) && (!packed || even)};
+  };
+  a.q = view(q, st, true);
+  a.k = view(k, st + 3, false);
+  a.v = view(v, st + 6, false);
+  a.dout = view(dout, st + 9, true);
   a.out = out, a.dq = dq, a.dk = dk, a.dv = dv, a.lse = lse, a.delta = delta;
   a.q_lens = q_lens, a.kv_lens = kv_lens, a.lens64 = lens64;
   a.b = b, a.sq = sq, a.sk = sk, a.hk = hk, a.g = g, a.hd = hd;

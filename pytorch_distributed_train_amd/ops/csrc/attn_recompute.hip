@@ -90,6 +90,8 @@ struct Args {
 __device__ const uint4 kZeros = {0, 0, 0, 0};
 __device__ const float kInf = INFINITY;
 
+DEV_INLINE int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 DEV_INLINE int length_of(const void* lens, int wide, int b, int most) {
   if (!lens) return most;
   long n = wide ? reinterpret_cast<const long*>(lens)[b]
@@ -102,7 +104,7 @@ struct Seq {
   int batch, kvh, qlen, klen, off;  // off = klen - qlen
   int rows;                         // qlen * g
   DEV_INLINE Seq(const Args& a, int bh) {
-    batch = bh / a.hk;
+    batch = uniform(bh / a.hk);
     kvh = bh - batch * a.hk;
     qlen = length_of(a.q_lens, a.lens64, batch, a.sq);
     klen = length_of(a.kv_lens, a.lens64, batch, a.sk);
@@ -118,14 +120,14 @@ struct Seq {
 DEV_INLINE void place(const Args& a, int nblk, bool last, int* bh, int* blk) {
   int heads = a.b * a.hk, i = blockIdx.x;
   if (a.causal) {
-    *blk = i / heads;
+    *blk = uniform(i / heads);
     *bh = i - *blk * heads;
     if (last) *blk = nblk - 1 - *blk;
   } else {
-    int grp = i / (8 * nblk), w = i - grp * 8 * nblk;
+    int grp = uniform(i / (8 * nblk)), w = i - grp * 8 * nblk;
     int n = heads - grp * 8;
     n = n < 8 ? n : 8;
-    *blk = w / n;
+    *blk = uniform(w / n);
     *bh = grp * 8 + w - *blk * n;
   }
 }
@@ -183,6 +185,10 @@ DEV_INLINE void to_lds16(const void* src, void* dst) {
 }
 // from the wave's `base` plus the lane's 32-bit offset
 DEV_INLINE void to_lds16(const void* base, unsigned off, void* dst) {
+  uintptr_t b = (uintptr_t)base;
+  b = (uintptr_t)(unsigned)uniform((int)(b >> 32)) << 32 |
+      (unsigned)uniform((int)b);
+  base = reinterpret_cast<const void*>(b);
   asm volatile(
       "s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
       :
@@ -198,16 +204,16 @@ DEV_INLINE void to_lds4(const void* src, void* dst) {
 }
 
 // A streamed operand: rows r0.. below `end` of one sequence and head go to
-// LDS in tiles of R rows, by 4 waves. PACKED: row r is position r / g of head
+// LDS in tiles of R rows, by W waves. PACKED: row r is position r / g of head
 // r % g, else position r. A wave's load moves RPI = 4 or 8 rows. In a whole
 // tile their addresses are a scalar base and a lane's offset that never
 // changes (`quick`: RPI rows must not straddle positions unevenly, so g
 // divides RPI or RPI g); lanes past the head's end fetch its first chunk,
 // whose partner in the product is 0 or whose result is not stored. The last
 // tile works out each lane's row and fetches zeros beyond the end.
-template <int HDT, int R, bool PACKED>
+template <int HDT, int R, bool PACKED, int W = 4>
 struct Stream {
-  static constexpr int NCH = Geo<HDT>::NCH, RPI = 64 / NCH, N = R / RPI / 4;
+  static constexpr int NCH = Geo<HDT>::NCH, RPI = 64 / NCH, N = R / RPI / W;
   static_assert(N > 0 && (NCH == 8 || N % 2 == 0), "pieces a wave");
   const char* base;
   long ss, sh;
@@ -300,6 +306,21 @@ DEV_INLINE void put_row(T* row, const f32x16* acc, float m, int hd, int lane) {
     }
 }
 
+// the same as fp32, 16 bytes a piece
+template <int DT>
+DEV_INLINE void put_part(float* row, const f32x16* acc, int hd, int lane) {
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      int d = dt * 32 + j * 8 + (lane >> 5) * 4;
+      if (d < hd)
+        *reinterpret_cast<float4*>(row + d) = {
+            acc[dt][4 * j], acc[dt][4 * j + 1], acc[dt][4 * j + 2],
+            acc[dt][4 * j + 3]};
+    }
+}
+
 DEV_INLINE float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
 DEV_INLINE s16x8 pack8(const unsigned* p) {
@@ -349,63 +370,42 @@ struct Row {
   }
 };
 
-// ---- forward: a block has 128 packed rows, a wave 32 ----------------------
+// what a lane carries of its row over the keys: P's reference, its sum and
+// O^T (lane: row, d = 32*i + 8*j + 4*h + 0..3)
 template <typename T, int HDT>
-__global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk) {
+struct Running {
   using G = Geo<HDT>;
-  LDS_BUFFER(k0, TILE * G::PITCH);
-  LDS_BUFFER(k1, TILE * G::PITCH);
-  LDS_BUFFER(v0, TILE * G::PITCH);
-  LDS_BUFFER(v1, TILE * G::PITCH);
-  int lane = threadIdx.x & 63, h = lane >> 5;
-  int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int bh, blk;
-  place(a, nblk, true, &bh, &blk);
-  Seq s(a, bh);
-  Row row(a, s, blk * 128 + wave * 32 + (lane & 31));
-  Stream<HDT, TILE, false> kin(a, a.k, s, lane), vin(a, a.v, s, lane);
-  s16x8 qf[G::KS];
-  keep<HDT>(a,
-            reinterpret_cast<const char*>(a.q.p) +
-                2 * (s.batch * a.q.sb + row.pos * a.q.ss + row.head * a.q.sh),
-            row.valid, lane, qf);
-  // keys that any row of the block sees: the last row's, or none
-  int last = (blk * 128 + 127) / a.g;
-  last = last < s.qlen ? last : s.qlen - 1;
-  int end = blk * 128 < s.rows ? s.klen : 0;
-  if (a.causal && last + s.off + 1 < end) end = last + s.off + 1;
-  int ntile = end > 0 ? (end + TILE - 1) / TILE : 0;
-  int wlo = wave_min(row.lim), whi = wave_max(row.valid ? row.lim : 0);
-
-  float c = a.scale * kLog2e, far = 8.f / c;
   float top = -INFINITY, sum = 0.f;
   f32x16 acc[G::DT];
+  float c, far;
+  DEV_INLINE explicit Running(float scale) : c(scale * kLog2e) {
+    far = 8.f / c;
 #pragma unroll
-  for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
-
-  auto load = [&](int t, char* kd, char* vd) {
-    kin.load(a, t * TILE, s.klen, kd, wave, lane);
-    vin.load(a, t * TILE, s.klen, vd, wave, lane);
-  };
-  auto step = [&](int t, const char* kt, const char* vt) {
-    int key0 = t * TILE;
-    if (key0 >= whi) return;
-    f32x16 sc[2] = {kNone, kNone};
+    for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
+  }
+  // keys key0 .. key0 + 32*U - 1; the lane's row sees those below `lim`,
+  // none of the wave's rows is cut short when they end below `wlo`
+  template <int U>
+  DEV_INLINE void step(const char* kt, const char* vt, const s16x8* qf,
+                       int key0, int lim, int wlo, int lane) {
+    f32x16 sc[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) sc[u] = kNone;
 #pragma unroll
     for (int ks = 0; ks < G::KS; ++ks)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < U; ++u)
         sc[u] = Op<T>::mfma(frag_row<HDT>(kt, u * 32, ks, lane), qf[ks],
                             sc[u]);
-    if (key0 + TILE > wlo) {
-      int rel = row.lim - key0 - h * 4;
+    if (key0 + U * 32 > wlo) {
+      int rel = lim - key0 - (lane >> 5) * 4;
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
+      for (int i = 0; i < U * 16; ++i)
         if ((i >> 2) * 8 + (i & 3) >= rel) sc[i >> 4][i & 15] = -INFINITY;
     }
     float m = sc[0][0];
 #pragma unroll
-    for (int i = 1; i < 32; ++i) m = fmaxf(m, sc[i >> 4][i & 15]);
+    for (int i = 1; i < U * 16; ++i) m = fmaxf(m, sc[i >> 4][i & 15]);
     m = fmaxf(m, other_half(m));
     // P is taken relative to `top`, which follows the running maximum only
     // when that is 2^8 past it: P stays below 2^8, which neither 16-bit type
@@ -421,9 +421,9 @@ __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk) {
         for (int j = 0; j < 16; ++j) acc[i][j] *= f;
     }
     float base = top == -INFINITY ? 0.f : -top * c;
-    unsigned p[16];
+    unsigned p[U * 8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < U * 8; ++i) {
       float x = __builtin_amdgcn_exp2f(
           fmaf(sc[i >> 3][(2 * i) & 15], c, base));
       float y = __builtin_amdgcn_exp2f(
@@ -432,15 +432,93 @@ __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk) {
       p[i] = Op<T>::pack(x, y);
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < U * 2; ++k)
 #pragma unroll
       for (int i = 0; i < G::DT; ++i)
         acc[i] = Op<T>::mfma(frag_col<HDT>(vt, k * 16, i, lane),
                              pack8(p + 4 * k), acc[i]);
+  }
+  // The row's output and lse; or, as part `at` of several (part: [parts]
+  // [rows][hd] of outputs, then [parts][rows] of lse, rows = b*hk*sq*g), its
+  // share of them for attn_rc_join_rows_k
+  DEV_INLINE void put(const Args& a, const Seq& s, const Row& row, int bh,
+                      int parts, int at, float* part, int lane) {
+    sum += other_half(sum);
+    if (!row.stored) return;
+    bool some = row.valid && row.lim > 0 && top != -INFINITY;
+    // a NaN has to come out: it fails the comparisons that raise `top`
+    some = some || (row.valid && sum != sum);
+    float lse = some ? top * c + __builtin_amdgcn_logf(sum) : INFINITY;
+    float m = some ? 1.f / sum : 0.f;
+    if (!some)
+#pragma unroll
+      for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
+    long r = (long)bh * a.sq * a.g + row.r;
+    if (parts == 1) {
+      T* o = reinterpret_cast<T*>(a.out) +
+             (((long)s.batch * a.sq + row.pos) * a.hk * a.g + row.head) *
+                 a.hd;
+      put_row<T, G::DT>(o, acc, m, a.hd, lane);
+      if (lane < 32 && a.lse) a.lse[r] = lse;
+      return;
+    }
+    long rows = (long)a.b * a.hk * a.sq * a.g;
+    if (lane < 32) part[parts * rows * a.hd + at * rows + r] = lse;
+    if (!some) return;  // not read then
+#pragma unroll
+    for (int i = 0; i < G::DT; ++i) acc[i] *= m;
+    put_part<G::DT>(part + (at * rows + r) * a.hd, acc, a.hd, lane);
+  }
+};
+
+// ---- forward: a block has 128 packed rows, a wave 32 ----------------------
+// nsplit > 1: the keys' tiles go in runs of `per` to that many blocks, whose
+// results a last kernel joins.
+template <typename T, int HDT>
+__global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk,
+                                                        int nsplit, int per,
+                                                        float* part) {
+  using G = Geo<HDT>;
+  LDS_BUFFER(k0, TILE * G::PITCH);
+  LDS_BUFFER(k1, TILE * G::PITCH);
+  LDS_BUFFER(v0, TILE * G::PITCH);
+  LDS_BUFFER(v1, TILE * G::PITCH);
+  int lane = threadIdx.x & 63;
+  int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int bh, blk;
+  place(a, nblk * nsplit, true, &bh, &blk);
+  int split = blk;
+  blk = uniform(blk / nsplit);
+  split -= blk * nsplit;
+  Seq s(a, bh);
+  Row row(a, s, blk * 128 + wave * 32 + (lane & 31));
+  Stream<HDT, TILE, false> kin(a, a.k, s, lane), vin(a, a.v, s, lane);
+  s16x8 qf[G::KS];
+  keep<HDT>(a,
+            reinterpret_cast<const char*>(a.q.p) +
+                2 * (s.batch * a.q.sb + row.pos * a.q.ss + row.head * a.q.sh),
+            row.valid, lane, qf);
+  // keys that any row of the block sees: the last row's, or none
+  int last = (blk * 128 + 127) / a.g;
+  last = last < s.qlen ? last : s.qlen - 1;
+  int end = blk * 128 < s.rows ? s.klen : 0;
+  if (a.causal && last + s.off + 1 < end) end = last + s.off + 1;
+  int ntile = end > 0 ? (end + TILE - 1) / TILE : 0;
+  int first = split * per;
+  if (nsplit > 1 && ntile > first + per) ntile = first + per;
+  int wlo = wave_min(row.lim), whi = wave_max(row.valid ? row.lim : 0);
+  Running<T, HDT> run(a.scale);
+  auto load = [&](int t, char* kd, char* vd) {
+    kin.load(a, t * TILE, s.klen, kd, wave, lane);
+    vin.load(a, t * TILE, s.klen, vd, wave, lane);
   };
-  if (ntile) load(0, k0, v0);
+  auto step = [&](int t, const char* kt, const char* vt) {
+    if (t * TILE < whi)
+      run.template step<2>(kt, vt, qf, t * TILE, row.lim, wlo, lane);
+  };
+  if (first < ntile) load(first, k0, v0);
   staged();
-  for (int t = 0; t < ntile; t += 2) {
+  for (int t = first; t < ntile; t += 2) {
     if (t + 1 < ntile) load(t + 1, k1, v1);
     step(t, k0, v0);
     staged();
@@ -449,23 +527,119 @@ __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk) {
     step(t + 1, k1, v1);
     staged();
   }
-  sum += other_half(sum);
-  if (!row.stored) return;
-  bool some = row.valid && row.lim > 0;
-  T* o = reinterpret_cast<T*>(a.out) +
-         (((long)s.batch * a.sq + row.pos) * a.hk * a.g + row.head) * a.hd;
-  if (!some)
-#pragma unroll
-    for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
-  put_row<T, G::DT>(o, acc, some ? 1.f / sum : 0.f, a.hd, lane);
-  if (h == 0 && a.lse)
-    a.lse[(long)bh * a.sq * a.g + row.r] =
-        some ? top * c + __builtin_amdgcn_logf(sum) : INFINITY;
+  run.put(a, s, row, bh, nsplit, split, part, lane);
+}
+
+// ---- forward of few rows (32 at most: single tokens) ----------------------
+// The keys' bytes are all there is to it, so every wave streams its own run
+// of them, 32 at a time, through its own two buffers, with no barrier: a
+// block's two waves share nothing but the launch. parts = 2 * gridDim / bh.
+template <typename T, int HDT>
+__global__ __launch_bounds__(128, 2) void attn_rc_few_k(Args a, int parts,
+                                                        int per,
+                                                        float* part) {
+  using G = Geo<HDT>;
+  using In = Stream<HDT, 32, false, 1>;
+  __shared__ __attribute__((aligned(16))) char lds[2][4][32 * G::PITCH];
+  int lane = threadIdx.x & 63;
+  int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int heads = a.b * a.hk;
+  int at = uniform(blockIdx.x / heads), bh = blockIdx.x - at * heads;
+  at = at * 2 + wave;
+  Seq s(a, bh);
+  Row row(a, s, lane & 31);
+  char *k0 = lds[wave][0], *v0 = lds[wave][1];
+  char *k1 = lds[wave][2], *v1 = lds[wave][3];
+  In kin(a, a.k, s, lane), vin(a, a.v, s, lane);
+  s16x8 qf[G::KS];
+  keep<HDT>(a,
+            reinterpret_cast<const char*>(a.q.p) +
+                2 * (s.batch * a.q.sb + row.pos * a.q.ss + row.head * a.q.sh),
+            row.valid, lane, qf);
+  int wlo = wave_min(row.lim), whi = wave_max(row.valid ? row.lim : 0);
+  int t = at * per, end = (whi + 31) / 32;
+  end = end < t + per ? end : t + per;
+  Running<T, HDT> run(a.scale);
+  auto load = [&](int i, char* kd, char* vd) {
+    kin.load(a, i * 32, s.klen, kd, 0, lane);
+    vin.load(a, i * 32, s.klen, vd, 0, lane);
+  };
+  // all but the newest tile's loads have landed
+  auto landed = [&](bool newest) {
+    if (newest)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * In::N) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  };
+  auto step = [&](int i, const char* kt, const char* vt) {
+    run.template step<1>(kt, vt, qf, i * 32, row.lim, wlo, lane);
+    // the buffer's reads are done before it is loaded again
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+  if (t < end) load(t, k0, v0);
+  for (; t < end; t += 2) {
+    if (t + 1 < end) load(t + 1, k1, v1);
+    landed(t + 1 < end);
+    step(t, k0, v0);
+    if (t + 1 >= end) break;
+    if (t + 2 < end) load(t + 2, k0, v0);
+    landed(t + 2 < end);
+    step(t + 1, k1, v1);
+  }
+  run.put(a, s, row, bh, parts, at, part, lane);
+}
+
+// out = sum over parts of exp2(lse_p - lse) out_p, lse = log2 sum exp2(lse_p);
+// 32 lanes a row. A part that saw no key has lse +inf and no output.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_rc_join_rows_k(Args a, int parts,
+                                                           const float* part) {
+  long rows = (long)a.b * a.hk * a.sq * a.g;
+  long r = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  int d = (threadIdx.x & 31) * 4;
+  const float* ls = part + parts * rows * a.hd + r;
+  float top = -INFINITY;
+  for (int p = 0; p < parts; ++p) {
+    float l = ls[p * rows];
+    if (l != INFINITY) top = fmaxf(top, l);
+  }
+  float sum = 0.f;
+  float4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < parts; ++p) {
+    float l = ls[p * rows];
+    if (l == INFINITY) continue;
+    float w = __builtin_amdgcn_exp2f(l - top);
+    sum += w;
+    if (d < a.hd) {
+      float4 x = *reinterpret_cast<const float4*>(part +
+                                                  (p * rows + r) * a.hd + d);
+      acc.x += w * x.x, acc.y += w * x.y, acc.z += w * x.z, acc.w += w * x.w;
+    }
+  }
+  float m = sum != 0.f ? 1.f / sum : 0.f;
+  int n = a.sq * a.g;
+  int bh = (int)(r / n), pr = (int)(r - (long)bh * n);
+  int batch = bh / a.hk, pos = (int)mdiv(pr, a.g_mul, a.g_shift);
+  int head = (bh - batch * a.hk) * a.g + pr - pos * a.g;
+  if (d < a.hd) {
+    uint2 v = {Op<T>::pack(acc.x * m, acc.y * m),
+               Op<T>::pack(acc.z * m, acc.w * m)};
+    *reinterpret_cast<uint2*>(
+        reinterpret_cast<T*>(a.out) +
+        (((long)batch * a.sq + pos) * a.hk * a.g + head) * a.hd + d) = v;
+  }
+  if (d == 0 && a.lse)
+    a.lse[r] = sum != 0.f ? top + __builtin_amdgcn_logf(sum) : INFINITY;
 }
 
 // ---- backward 1: D, and dQ of 128 packed rows -----------------------------
+// nsplit > 1: the keys' tiles go to that many blocks in turn, whose fp32 sums
+// a last kernel adds.
 template <typename T, int HDT>
-__global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk) {
+__global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk,
+                                                       int nsplit,
+                                                       float* part) {
   using G = Geo<HDT>;
   LDS_BUFFER(k0, TILE * G::PITCH);
   LDS_BUFFER(k1, TILE * G::PITCH);
@@ -474,7 +648,10 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk) {
   int lane = threadIdx.x & 63, h = lane >> 5;
   int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int bh, blk;
-  place(a, nblk, true, &bh, &blk);
+  place(a, nblk * nsplit, true, &bh, &blk);
+  int split = blk;
+  blk = uniform(blk / nsplit);
+  split -= blk * nsplit;
   Seq s(a, bh);
   Row row(a, s, blk * 128 + wave * 32 + (lane & 31));
   Stream<HDT, TILE, false> kin(a, a.k, s, lane), vin(a, a.v, s, lane);
@@ -488,7 +665,7 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk) {
     kin.load(a, t * TILE, s.klen, kd, wave, lane);
     vin.load(a, t * TILE, s.klen, vd, wave, lane);
   };
-  if (ntile) load(0, k0, v0);
+  if (split < ntile) load(split, k0, v0);
   s16x8 qf[G::KS], df[G::KS];
   keep<HDT>(a,
             reinterpret_cast<const char*>(a.dout.p) +
@@ -518,7 +695,7 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk) {
   float lse = INFINITY;
   long lat = (long)bh * a.sq * a.g + row.r;
   if (row.valid) lse = a.lse[lat];
-  if (row.stored && h == 0) a.delta[lat] = delta;
+  if (row.stored && h == 0 && split == 0) a.delta[lat] = delta;
 
   float c = a.scale * kLog2e;
   f32x16 acc[G::DT];
@@ -559,13 +736,14 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk) {
     }
   };
   staged();
-  for (int t = 0; t < ntile; t += 2) {
-    if (t + 1 < ntile) load(t + 1, k1, v1);
+  for (int t = split; t < ntile; t += 2 * nsplit) {
+    int t1 = t + nsplit, t2 = t1 + nsplit;
+    if (t1 < ntile) load(t1, k1, v1);
     step(t, k0, v0);
     staged();
-    if (t + 1 >= ntile) break;
-    if (t + 2 < ntile) load(t + 2, k0, v0);
-    step(t + 1, k1, v1);
+    if (t1 >= ntile) break;
+    if (t2 < ntile) load(t2, k0, v0);
+    step(t1, k1, v1);
     staged();
   }
   if (!row.stored) return;
@@ -573,8 +751,13 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk) {
   if (!some)
 #pragma unroll
     for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
-  put_row<T, G::DT>(reinterpret_cast<T*>(a.dq) + oat, acc, a.scale, a.hd,
-                    lane);
+  if (nsplit == 1) {
+    put_row<T, G::DT>(reinterpret_cast<T*>(a.dq) + oat, acc, a.scale, a.hd,
+                      lane);
+    return;
+  }
+  put_part<G::DT>(part + (long)split * a.b * a.sq * a.hk * a.g * a.hd + oat,
+                  acc, a.hd, lane);
 }
 
 // ---- backward 2: dK, dV of 128 keys, over all packed rows -----------------
@@ -601,8 +784,9 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
   int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int bh, blk;
   place(a, nblk * nsplit, false, &bh, &blk);
-  int split = blk % nsplit;
-  blk /= nsplit;
+  int split = blk;
+  blk = uniform(blk / nsplit);
+  split -= blk * nsplit;
   Seq s(a, bh);
   int key = blk * 128 + wave * 32 + (lane & 31);
   bool valid = key < s.klen;
@@ -729,69 +913,101 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
   }
   long n = (long)a.b * a.sk * a.hk * a.hd;
   float* out = part + 2 * split * n + at;
-#pragma unroll
-  for (int i = 0; i < G::DT; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      int e = i * 32 + j * 8 + h * 4;
-      if (e < a.hd) {
-        *reinterpret_cast<float4*>(out + e) = {dk[i][4 * j], dk[i][4 * j + 1],
-                                               dk[i][4 * j + 2],
-                                               dk[i][4 * j + 3]};
-        *reinterpret_cast<float4*>(out + n + e) = {
-            dv[i][4 * j], dv[i][4 * j + 1], dv[i][4 * j + 2],
-            dv[i][4 * j + 3]};
-      }
-    }
+  put_part<G::DT>(out, dk, a.hd, lane);
+  put_part<G::DT>(out + n, dv, a.hd, lane);
 }
 
-// dk, dv = sums over the splits' part[split][2][n], 4 elements a thread
+// x, y = sums over the splits of part[split][x then y], x times `scale`;
+// 4 elements a thread; nx and ny are multiples of 4
 template <typename T>
 __global__ __launch_bounds__(256) void attn_rc_join_k(
-    const float* __restrict__ part, long n, int nsplit, float scale,
-    T* __restrict__ dk, T* __restrict__ dv) {
+    const float* __restrict__ part, long nx, long ny, int nsplit, float scale,
+    T* __restrict__ x, T* __restrict__ y) {
   long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= 2 * n) return;
+  if (i >= nx + ny) return;
   float4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int k = 0; k < nsplit; ++k) {
-    float4 x = *reinterpret_cast<const float4*>(part + 2 * k * n + i);
-    sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+    float4 v = *reinterpret_cast<const float4*>(part + k * (nx + ny) + i);
+    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
   }
-  float m = i < n ? scale : 1.f;
+  float m = i < nx ? scale : 1.f;
   uint2 v = {Op<T>::pack(sum.x * m, sum.y * m),
              Op<T>::pack(sum.z * m, sum.w * m)};
-  *reinterpret_cast<uint2*>(i < n ? dk + i : dv + (i - n)) = v;
+  *reinterpret_cast<uint2*>(i < nx ? x + i : y + (i - nx)) = v;
 }
 
-// Blocks that share a key block's rows. Two blocks run on each of 256 CUs;
-// below four rounds of them (a causal mask's blocks differ in length) rows
-// are dealt out, 512 at least to each.
-int dkv_splits(long b, long sq, long sk, long hk, long g) {
-  long blocks = b * hk * ((sk + 127) / 128), rows = sq * g;
-  if (blocks == 0) return 1;
-  long n = (2048 + blocks - 1) / blocks;
-  if (n > rows / 512) n = rows / 512;
-  if (n > 16) n = 16;
-  return n < 1 ? 1 : (int)n;
-}
+// How work is dealt out where there are few blocks; shapes alone decide. Two
+// blocks run on each of 256 CUs.
+struct Plan {
+  int fwd, per;  // forward: parts over the keys, tiles of each
+  bool few;      // rows fit one wave: attn_rc_few_k, tiles of 32
+  int dq, dkv;   // backward: parts over the keys, over the rows
+  Plan(long b, long sq, long sk, long hk, long g) {
+    long bh = b * hk, rows = sq * g;
+    long rblk = bh * ((rows + 127) / 128), kblk = bh * ((sk + 127) / 128);
+    fwd = dq = dkv = 1;
+    per = 0;
+    few = false;
+    if (rblk == 0 || kblk == 0) return;
+    if (rows <= 32 && sk >= 512) {
+      // runs of 256 keys (8 tiles) a wave, longer where that makes more
+      // than 4096 waves, 128 where it makes fewer than 1024
+      few = true;
+      long tiles = (sk + 31) / 32, run = 8;
+      if (bh * ((tiles + 7) / 8) < 1024) run = 4;
+      while (run < tiles && bh * ((tiles + run - 1) / run) > 4096) run *= 2;
+      per = (int)run;
+      fwd = (int)((tiles + 2 * run - 1) / (2 * run)) * 2;
+    } else {
+      long tiles = (sk + TILE - 1) / TILE;
+      fwd = clamp(1024 / rblk, tiles / 8);
+      per = (int)((tiles + fwd - 1) / fwd);
+    }
+    dq = clamp(1024 / rblk, sk / 512);
+    // a causal mask's blocks differ in length: more rounds even them out
+    dkv = clamp((1024 + kblk - 1) / kblk, rows / 512);
+  }
+  static int clamp(long want, long most) {
+    long n = want < most ? want : most;
+    n = n < 16 ? n : 16;
+    return n < 1 ? 1 : (int)n;
+  }
+};
 
 template <typename T, int HDT>
-void launch(const Args& a, int bwd, float* part, hipStream_t s) {
+void launch(const Args& a, int bwd, float* ws, hipStream_t s) {
   int rblk = (a.sq * a.g + 127) / 128, kblk = (a.sk + 127) / 128;
   int bh = a.b * a.hk;
+  Plan p(a.b, a.sq, a.sk, a.hk, a.g);
   if (!bwd) {
-    if (rblk) attn_rc_fwd_k<T, HDT><<<bh * rblk, 256, 0, s>>>(a, rblk);
+    if (rblk == 0) return;
+    if (p.few)
+      attn_rc_few_k<T, HDT>
+          <<<bh * (p.fwd / 2), 128, 0, s>>>(a, p.fwd, p.per, ws);
+    else
+      attn_rc_fwd_k<T, HDT>
+          <<<bh * rblk * p.fwd, 256, 0, s>>>(a, rblk, p.fwd, p.per, ws);
+    if (p.fwd > 1) {
+      long rows = (long)bh * a.sq * a.g;
+      attn_rc_join_rows_k<T><<<(rows + 7) / 8, 256, 0, s>>>(a, p.fwd, ws);
+    }
     return;
   }
-  if (rblk) attn_rc_dq_k<T, HDT><<<bh * rblk, 256, 0, s>>>(a, rblk);
-  if (!kblk) return;
-  int nsplit = dkv_splits(a.b, a.sq, a.sk, a.hk, a.g);
-  attn_rc_dkv_k<T, HDT><<<bh * kblk * nsplit, 256, 0, s>>>(a, kblk, nsplit,
-                                                           part);
-  if (nsplit > 1) {
-    long n = (long)a.b * a.sk * a.hk * a.hd;
-    attn_rc_join_k<T><<<(n / 2 + 255) / 256, 256, 0, s>>>(
-        part, n, nsplit, a.scale, (T*)a.dk, (T*)a.dv);
+  long nq = (long)a.b * a.sq * a.hk * a.g * a.hd;
+  long nk = (long)a.b * a.sk * a.hk * a.hd;
+  if (rblk) {
+    attn_rc_dq_k<T, HDT><<<bh * rblk * p.dq, 256, 0, s>>>(a, rblk, p.dq, ws);
+    if (p.dq > 1)
+      attn_rc_join_k<T><<<(nq / 4 + 255) / 256, 256, 0, s>>>(
+          ws, nq, 0, p.dq, a.scale, (T*)a.dq, nullptr);
+  }
+  if (kblk) {
+    attn_rc_dkv_k<T, HDT>
+        <<<bh * kblk * p.dkv, 256, 0, s>>>(a, kblk, p.dkv, ws);
+    if (p.dkv > 1)
+      attn_rc_join_k<T><<<(nk / 2 + 255) / 256, 256, 0, s>>>(
+          ws, nk, nk, p.dkv, a.scale, (T*)a.dk, (T*)a.dv);
   }
 }
 
@@ -799,17 +1015,20 @@ void launch(const Args& a, int bwd, float* part, hipStream_t s) {
 
 extern "C" {
 
-// floats of workspace that backward needs
+// floats of workspace that forward or backward needs
 long pdta_attn_recompute_ws(long b, long sq, long sk, long hk, long g,
-                            long hd) {
-  int n = dkv_splits(b, sq, sk, hk, g);
-  return n > 1 ? 2 * n * b * sk * hk * hd : 0;
+                            long hd, int bwd) {
+  Plan p(b, sq, sk, hk, g);
+  long nq = b * sq * hk * g * hd, nk = b * sk * hk * hd;
+  if (!bwd) return p.fwd > 1 ? p.fwd * (nq + nq / hd) : 0;
+  long x = p.dq > 1 ? p.dq * nq : 0, y = p.dkv > 1 ? 2 * p.dkv * nk : 0;
+  return x > y ? x : y;
 }
 
 // strides: q, k, v, dout, each (b, s, head) in elements; multiples of 8, all
 // pointers 16-byte aligned, hd a multiple of 8 up to 128. lens null or [b].
 // Forward writes out and, unless null, lse; backward reads both and writes
-// delta, dq, dk, dv, with pdta_attn_recompute_ws floats in ws. Grids must stay below 2^31 blocks and sq*g below 2^31.
+// delta, dq, dk, dv; either with pdta_attn_recompute_ws floats in ws. Grids must stay below 2^31 blocks and sq*g below 2^31.
 void pdta_attn_recompute(const void* q, const void* k, const void* v,
                          const void* dout, const long* st, void* out,
                          float* lse, float* delta, void* dq, void* dk,

@@ -25,7 +25,7 @@ void pdta_attn_recompute(const void*, const void*, const void*, const void*,
                          void*, const void*, const void*, int, int, int, int,
                          int, int, int, float, int, int, float*, int,
                          hipStream_t);
-long pdta_attn_recompute_ws(long, long, long, long, long, long);
+long pdta_attn_recompute_ws(long, long, long, long, long, long, int);
 }
 
 namespace {
@@ -330,13 +330,18 @@ std::vector<at::Tensor> attn_recompute_fwd(
   attn_strides(k, st + 3);
   attn_strides(v, st + 6);
   if (out.numel()) {
+    long need =
+        pdta_attn_recompute_ws(n.b, n.sq, n.sk, n.hk, g, n.hd, 0);
+    at::Tensor ws;
+    if (need) ws = at::empty({need}, lse.options());
     pdta_attn_recompute(q.data_ptr(), k.data_ptr(), v.data_ptr(), nullptr,
                         st, out.data_ptr(),
                         want_lse ? lse.data_ptr<float>() : nullptr, nullptr,
                         nullptr, nullptr, nullptr, len_ptr(q_lens),
                         len_ptr(kv_lens), lens_wide(q_lens, kv_lens), n.b,
                         n.sq, n.sk, n.hk, g, n.hd, (float)scale, causal, 0,
-                        nullptr, dt_of(q), cur_stream());
+                        need ? ws.data_ptr<float>() : nullptr, dt_of(q),
+                        cur_stream());
     launched("attn_recompute_fwd");
   }
   return {out, lse};
@@ -368,7 +373,7 @@ std::vector<at::Tensor> attn_recompute_bwd(
   auto dv = at::empty_like(dk);
   auto delta = at::empty_like(lse);
   auto ws = at::empty(
-      {pdta_attn_recompute_ws(n.b, n.sq, n.sk, n.hk, g, n.hd)},
+      {pdta_attn_recompute_ws(n.b, n.sq, n.sk, n.hk, g, n.hd, 1)},
       lse.options());
   long st[12];
   attn_strides(q, st);

@@ -138,6 +138,13 @@ CASES = [
     (1, 700, 1100, 2, 1, 64, True, None, None),
     (1, 1025, 1025, 4, 2, 128, True, None, None),
     (3, 5, 2000, 2, 1, 128, True, None, [2000, 3, 777]),
+    # few rows against many keys, which are dealt out and joined
+    (2, 1, 1000, 3, 3, 64, False, None, [0, 999]),
+    (4, 3, 900, 6, 2, 96, True, [3, 0, 2, 1], [900, 5, 0, 513]),
+    (1, 32, 600, 1, 1, 80, True, None, None),
+    (1, 8, 515, 8, 2, 128, False, None, None),
+    (1, 2, 9000, 3, 1, 64, True, None, None),
+    (2100, 1, 512, 2, 2, 8, False, None, None),
 ]
 
 
@@ -195,21 +202,23 @@ def test_gradients_against_differences(causal, ql, kl):
 def test_what_lies_behind_a_sequence_is_not_read(dtype, bad):
     if bad == "lowest":
         bad = torch.finfo(dtype).min
-    b, s, h, hk, hd = 4, 150, 4, 2, 128
     lens = [0, 1, 70, 129]
-    q, k, v, do = _inputs("cuda", dtype, b, s, s, h, hk, hd, seed=5)
-    want = _run(q, k, v, do, q_lens=_t(lens, "cuda"),
-                kv_lens=_t(lens, "cuda"))
-    for i, n in enumerate(lens):
-        for x in (q, k, v, do):
-            x[i, n:] = bad
-    got = _run(q, k, v, do, q_lens=_t(lens, "cuda"),
-               kv_lens=_t(lens, "cuda"))
-    for u, w in zip(got, want):
-        assert torch.equal(u, w)
-    for i, n in enumerate(lens):
-        for u in got:
-            assert bool((u[i, n:] == 0).all())
+    for sq, sk, hd, ql, kl in ((150, 150, 128, lens, lens),
+                               (150, 150, 40, lens, lens),
+                               (6, 700, 64, [6, 0, 1, 3],
+                                [0, 1, 600, 699])):
+        q, k, v, do = _inputs("cuda", dtype, 4, sq, sk, 4, 2, hd, seed=5)
+        kw = {"q_lens": _t(ql, "cuda"), "kv_lens": _t(kl, "cuda")}
+        want = _run(q, k, v, do, **kw)
+        for i in range(4):
+            q[i, ql[i]:] = do[i, ql[i]:] = bad
+            k[i, kl[i]:] = v[i, kl[i]:] = bad
+        got = _run(q, k, v, do, **kw)
+        for u, w in zip(got, want):
+            assert torch.equal(u, w)
+        for i in range(4):
+            for u, n in zip(got, (ql, ql, kl, kl)):
+                assert bool((u[i, n[i]:] == 0).all())
 
 
 @gpu

@@ -25,10 +25,16 @@
 // lanes outside a sequence or past the head's end fetch zeros, so nothing
 // behind a sequence is ever read.
 //
-// LDS rows are 128 or 256 bytes; 16-byte chunk c of row r lies at
-// c ^ perm(r), perm(r) = r's bits (1,0,2): 8 neighbouring rows spread over
-// all banks both for row fragments (16 bytes of one row a lane) and for the
-// transposing reads, whose 4 rows x 32 bytes need different chunk pairs.
+// LDS rows are 128 or 256 bytes, in groups of 1024 bytes (what one load
+// brings) that lie 1056 or 1040 apart; 16-byte chunk c of row r lies at
+// c ^ perm(r). The banks span 256 bytes, and a row fragment's read (16 bytes
+// of a row a lane) is served 16 lanes at a time, lanes 0-3, 12-15, 20-27 and
+// the rest: these rows need 16 different 16-byte places. The transposing
+// reads take 64 bytes of 4 neighbouring rows at a time: these need 4
+// different 64-byte places. perm puts a row's low bits into the place's high
+// bits for the latter, the bytes between groups set the others apart for the
+// former, and the way from row to row + 16 stays a constant. Conflicts took
+// 16 to 20% of all cycles at heads of 128 when perm alone did this.
 #include "common.h"
 
 namespace {
@@ -134,37 +140,50 @@ DEV_INLINE void place(const Args& a, int nblk, bool last, int* bh, int* blk) {
 
 template <int HDT> struct Geo {
   static constexpr int NCH = HDT == 64 ? 8 : 16;  // chunks of an LDS row
-  static constexpr int PITCH = NCH * 16;
+  static constexpr int GROUP = 64 / NCH;          // rows of a group
+  static constexpr int SPAN = HDT == 64 ? 1056 : 1040;
+  static constexpr int bytes(int rows) { return rows / GROUP * SPAN; }
   static constexpr int KS = HDT / 16;  // k steps of a product over the head
   static constexpr int DT = HDT / 32;  // 32-column tiles of the head
 };
 
-DEV_INLINE int perm(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+template <int HDT>
+DEV_INLINE int perm(int row) {
+  return HDT == 64 ? ((row & 2) << 1) | ((row & 4) >> 2) : (row & 3) << 2;
+}
+template <int HDT>
+DEV_INLINE int lds_at(int row, int chunk) {
+  using G = Geo<HDT>;
+  return row / G::GROUP * G::SPAN + row % G::GROUP * (G::NCH * 16) +
+         ((chunk ^ perm<HDT>(row)) << 4);
+}
 
 // A or B operand whose k runs along the row: rows r0 + (lane & 31), elements
-// 16*ks + 8*(lane >> 5) + 0..7
+// 16*ks + 8*(lane >> 5) + 0..7; r0 a multiple of 16
 template <int HDT>
 DEV_INLINE s16x8 frag_row(const char* lds, int r0, int ks, int lane) {
   return *reinterpret_cast<const s16x8*>(
-      lds + (r0 + (lane & 31)) * Geo<HDT>::PITCH +
-      (((2 * ks + (lane >> 5)) ^ perm(lane)) << 4));
+      lds + Geo<HDT>::bytes(r0) +
+      lds_at<HDT>(lane & 31, 2 * ks + (lane >> 5)));
 }
 
+DEV_INLINE s16x8 read_tr2(const char* lo, const char* hi) {
+  typedef __attribute__((address_space(3))) s16x4* tp_t;
+  s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tp_t)lo);
+  s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tp_t)hi);
+  return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+}
 // A operand whose k runs down the rows, in the accumulators' order: column
 // 32*dt + (lane & 31), rows r0 + 4*h + 0..3 and r0 + 8 + 4*h + 0..3 with
-// h = lane >> 5. The transposing read hands each lane of 16 one column of
-// the 4 x 16 block that the 16 lanes fetch in 8-byte pieces.
+// h = lane >> 5; r0 a multiple of 16. The transposing read hands each lane of
+// 16 one column of the 4 x 16 block that the 16 lanes fetch in 8-byte pieces.
 template <int HDT>
 DEV_INLINE s16x8 frag_col(const char* lds, int r0, int dt, int lane) {
   int row = 4 * (lane >> 5) + ((lane >> 2) & 3);
   int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1);
-  const char* p = lds + (r0 + row) * Geo<HDT>::PITCH +
-                  ((chunk ^ perm(row)) << 4) + (lane & 1) * 8;
-  typedef __attribute__((address_space(3))) s16x4* tp_t;
-  s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tp_t)p);
-  s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (tp_t)(p + 8 * Geo<HDT>::PITCH));
-  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  const char* p = lds + Geo<HDT>::bytes(r0) + lds_at<HDT>(row, chunk) +
+                  (lane & 1) * 8;
+  return read_tr2(p, p + Geo<HDT>::bytes(8));
 }
 
 // Global to LDS: lane l's 16 (4) bytes land at dst + 16 (4) * l. In assembly
@@ -214,10 +233,11 @@ DEV_INLINE void to_lds4(const void* src, void* dst) {
 template <int HDT, int R, bool PACKED, int W = 4>
 struct Stream {
   static constexpr int NCH = Geo<HDT>::NCH, RPI = 64 / NCH, N = R / RPI / W;
-  static_assert(N > 0 && (NCH == 8 || N % 2 == 0), "pieces a wave");
+  static_assert(N > 0, "pieces a wave");
+  static constexpr int SPAN = Geo<HDT>::SPAN;
   const char* base;
   long ss, sh;
-  unsigned off[2];  // even and odd pieces (their rows' perm differs)
+  unsigned off;
   bool quick;
 
   DEV_INLINE Stream(const Args& a, const View& v, const Seq& s, int lane) {
@@ -225,14 +245,11 @@ struct Stream {
     base = reinterpret_cast<const char*>(v.p) +
            2 * (s.batch * v.sb + (long)s.kvh * (PACKED ? a.g : 1) * sh);
     quick = v.quick;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      int l = lane / NCH;
-      int chunk = (lane % NCH) ^ perm(NCH == 8 ? l : l + 4 * k);
-      if (chunk * 8 >= a.hd) chunk = 0;
-      long at = PACKED ? (l / a.g) * ss + (l % a.g) * sh : l * ss;
-      off[k] = (unsigned)(2 * at) + chunk * 16;
-    }
+    int l = lane / NCH;
+    int chunk = (lane % NCH) ^ perm<HDT>(l);
+    if (chunk * 8 >= a.hd) chunk = 0;
+    long at = PACKED ? (l / a.g) * ss + (l % a.g) * sh : l * ss;
+    off = (unsigned)(2 * at) + chunk * 16;
   }
 
   DEV_INLINE void load(const Args& a, int r0, int end, char* lds, int wave,
@@ -248,7 +265,7 @@ struct Stream {
         } else {
           at = x * ss;
         }
-        to_lds16(base + 2 * at, off[NCH == 8 ? 0 : i & 1], lds + idx * 1024);
+        to_lds16(base + 2 * at, off, lds + idx * SPAN);
       }
       return;
     }
@@ -257,7 +274,7 @@ struct Stream {
     for (int i = 0; i < N; ++i) {
       int idx = wave * N + i;
       int row = idx * RPI + lane / NCH;
-      int chunk = (lane % NCH) ^ perm(row);
+      int chunk = (lane % NCH) ^ perm<HDT>(row);
       int r = r0 + row;
       long at;
       if (PACKED) {
@@ -269,7 +286,7 @@ struct Stream {
       const char* src = base + 2 * at + chunk * 16;
       if (r >= end || chunk * 8 >= a.hd)
         src = reinterpret_cast<const char*>(&kZeros);
-      to_lds16(src, lds + idx * 1024);
+      to_lds16(src, lds + idx * SPAN);
     }
   }
 };
@@ -479,10 +496,10 @@ __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk,
                                                         int nsplit, int per,
                                                         float* part) {
   using G = Geo<HDT>;
-  LDS_BUFFER(k0, TILE * G::PITCH);
-  LDS_BUFFER(k1, TILE * G::PITCH);
-  LDS_BUFFER(v0, TILE * G::PITCH);
-  LDS_BUFFER(v1, TILE * G::PITCH);
+  LDS_BUFFER(k0, G::bytes(TILE));
+  LDS_BUFFER(k1, G::bytes(TILE));
+  LDS_BUFFER(v0, G::bytes(TILE));
+  LDS_BUFFER(v1, G::bytes(TILE));
   int lane = threadIdx.x & 63;
   int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int bh, blk;
@@ -540,7 +557,7 @@ __global__ __launch_bounds__(128, 2) void attn_rc_few_k(Args a, int parts,
                                                         float* part) {
   using G = Geo<HDT>;
   using In = Stream<HDT, 32, false, 1>;
-  __shared__ __attribute__((aligned(16))) char lds[2][4][32 * G::PITCH];
+  __shared__ __attribute__((aligned(16))) char lds[2][4][G::bytes(32)];
   int lane = threadIdx.x & 63;
   int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int heads = a.b * a.hk;
@@ -641,10 +658,10 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk,
                                                        int nsplit,
                                                        float* part) {
   using G = Geo<HDT>;
-  LDS_BUFFER(k0, TILE * G::PITCH);
-  LDS_BUFFER(k1, TILE * G::PITCH);
-  LDS_BUFFER(v0, TILE * G::PITCH);
-  LDS_BUFFER(v1, TILE * G::PITCH);
+  LDS_BUFFER(k0, G::bytes(TILE));
+  LDS_BUFFER(k1, G::bytes(TILE));
+  LDS_BUFFER(v0, G::bytes(TILE));
+  LDS_BUFFER(v1, G::bytes(TILE));
   int lane = threadIdx.x & 63, h = lane >> 5;
   int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int bh, blk;
@@ -674,8 +691,9 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk,
             row.valid, lane, df);
   long oat = (((long)s.batch * a.sq + row.pos) * a.hk * a.g + row.head) *
              a.hd;
-  // D from the stored output: its rounding moves dS by P times a sum of
-  // random half steps, below dS's own rounding
+  // D from the stored output. Its rounding moves dS by P times a sum of
+  // random half steps, which is below dS's own rounding where P is spread
+  // over many keys; rows of few keys get it from P and dP, below.
   keep<HDT>(a, reinterpret_cast<const char*>(a.out) + 2 * oat, row.valid,
             lane, qf);
   float delta = 0.f;
@@ -695,38 +713,42 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk,
   float lse = INFINITY;
   long lat = (long)bh * a.sq * a.g + row.r;
   if (row.valid) lse = a.lse[lat];
-  if (row.stored && h == 0 && split == 0) a.delta[lat] = delta;
 
   float c = a.scale * kLog2e;
   f32x16 acc[G::DT];
 #pragma unroll
   for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
+  // P and dP of keys key0.. that lie at rows r0.. of the tiles
+  auto probs = [&](const char* kt, const char* vt, int r0, int key0,
+                   f32x16& sc, f32x16& dp) {
+    sc = dp = kNone;
+#pragma unroll
+    for (int ks = 0; ks < G::KS; ++ks) {
+      sc = Op<T>::mfma(frag_row<HDT>(kt, r0, ks, lane), qf[ks], sc);
+      dp = Op<T>::mfma(frag_row<HDT>(vt, r0, ks, lane), df[ks], dp);
+    }
+    if (key0 + 32 > wlo) {
+      int rel = row.lim - key0 - h * 4;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if ((i >> 2) * 8 + (i & 3) >= rel) sc[i] = -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], c, -lse));
+  };
   auto step = [&](int t, const char* kt, const char* vt) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       int key0 = t * TILE + u * 32;
       if (key0 >= whi) return;
-      f32x16 sc = kNone, dp = kNone;
-#pragma unroll
-      for (int ks = 0; ks < G::KS; ++ks) {
-        sc = Op<T>::mfma(frag_row<HDT>(kt, u * 32, ks, lane), qf[ks], sc);
-        dp = Op<T>::mfma(frag_row<HDT>(vt, u * 32, ks, lane), df[ks], dp);
-      }
-      if (key0 + 32 > wlo) {
-        int rel = row.lim - key0 - h * 4;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if ((i >> 2) * 8 + (i & 3) >= rel) sc[i] = -INFINITY;
-      }
+      f32x16 x, dp;
+      probs(kt, vt, u * 32, key0, x, dp);
       unsigned p[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float x = __builtin_amdgcn_exp2f(fmaf(sc[2 * i], c, -lse)) *
-                  (dp[2 * i] - delta);
-        float y = __builtin_amdgcn_exp2f(fmaf(sc[2 * i + 1], c, -lse)) *
-                  (dp[2 * i + 1] - delta);
-        p[i] = Op<T>::pack(x, y);
-      }
+      for (int i = 0; i < 8; ++i)
+        p[i] = Op<T>::pack(x[2 * i] * (dp[2 * i] - delta),
+                           x[2 * i + 1] * (dp[2 * i + 1] - delta));
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -736,6 +758,19 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk,
     }
   };
   staged();
+  if (split == 0 && ntile > 0 && wlo <= TILE) {
+    float d = 0.f;
+#pragma unroll 1
+    for (int u = 0; u < 2; ++u) {
+      f32x16 x, dp;
+      probs(k0, v0, u * 32, u * 32, x, dp);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) d += x[i] * dp[i];
+    }
+    d += other_half(d);
+    if (row.lim <= TILE) delta = row.valid ? d : 0.f;
+  }
+  if (row.stored && h == 0 && split == 0) a.delta[lat] = delta;
   for (int t = split; t < ntile; t += 2 * nsplit) {
     int t1 = t + nsplit, t2 = t1 + nsplit;
     if (t1 < ntile) load(t1, k1, v1);
@@ -773,13 +808,13 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
   using G = Geo<HDT>;
   constexpr bool VLDS = HDT > 64;
   constexpr int RT = VLDS ? 32 : 64;
-  LDS_BUFFER(q0, RT * G::PITCH);
-  LDS_BUFFER(q1, RT * G::PITCH);
-  LDS_BUFFER(d0, RT * G::PITCH);
-  LDS_BUFFER(d1, RT * G::PITCH);
+  LDS_BUFFER(q0, G::bytes(RT));
+  LDS_BUFFER(q1, G::bytes(RT));
+  LDS_BUFFER(d0, G::bytes(RT));
+  LDS_BUFFER(d1, G::bytes(RT));
   LDS_BUFFER(stat0, 512);  // 64 rows' lse and D
   LDS_BUFFER(stat1, 512);
-  LDS_BUFFER(vkeep, VLDS ? 128 * G::PITCH : 16);
+  LDS_BUFFER(vkeep, VLDS ? G::bytes(128) : 16);
   int lane = threadIdx.x & 63, h = lane >> 5;
   int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int bh, blk;
@@ -917,6 +952,202 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
   put_part<G::DT>(out + n, dv, a.hd, lane);
 }
 
+// ---- backward of short sequences: all three gradients in one pass ---------
+// 65 to 256 keys, as many packed rows, heads up to 64: a block of 8 waves
+// holds a key head's keys, 32 a wave, and runs over its rows 32 at a time, so
+// S, dP and the exponentials are worked out once and q, k, v, out and dout
+// are read once, all at the start: a step is shorter than a load's latency.
+// dK and dV gather in registers as in attn_rc_dkv_k. dQ needs all keys of a
+// row: the waves put dS (16 bits, which it has as an operand anyway) to LDS,
+// and after the step's one barrier each takes a 16 x 16 piece of dQ over all
+// keys, K^T kept in registers. dS rows are one key's 32 rows, 64 bytes;
+// 8-byte piece (j, h) lies at (j ^ perm2(key), h ^ key bit 3): 16 keys'
+// writes and the transposing reads' 4 keys x 32 bytes meet distinct banks.
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+DEV_INLINE int perm2(int key) {
+  return (((key >> 1) & 1) << 1) | ((key >> 2) & 1);
+}
+template <typename T> DEV_INLINE f32x4v mfma16(s16x8 a, s16x8 b, f32x4v c);
+template <>
+DEV_INLINE f32x4v mfma16<__hip_bfloat16>(s16x8 a, s16x8 b, f32x4v c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+      __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+      0);
+}
+template <>
+DEV_INLINE f32x4v mfma16<__half>(s16x8 a, s16x8 b, f32x4v c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(
+      __builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <typename T>
+__global__ __launch_bounds__(512, 2) void attn_rc_bwd_short_k(Args a) {
+  LDS_BUFFER(qall, Geo<64>::bytes(256));
+  LDS_BUFFER(dall, Geo<64>::bytes(256));
+  LDS_BUFFER(ds01, Geo<64>::bytes(256));  // two steps' dS; first K, all of it
+  __shared__ float lse[256], del[256];
+  int lane = threadIdx.x & 63, h = lane >> 5;
+  int wave = uniform(threadIdx.x >> 6);
+  int bh = blockIdx.x;
+  Seq s(a, bh);
+  int key = wave * 32 + (lane & 31);
+  bool valid = key < s.klen;
+  bool cut = wave_max(!valid) != 0, live = wave * 32 < s.klen;
+  int ntile = (s.rows + 31) / 32;
+  Stream<64, 256, false, 8> kin(a, a.k, s, lane);
+  Stream<64, 256, true, 8> qin(a, a.q, s, lane), din(a, a.dout, s, lane);
+  kin.load(a, 0, s.klen, ds01, wave, lane);
+  qin.load(a, 0, s.rows, qall, wave, lane);
+  din.load(a, 0, s.rows, dall, wave, lane);
+  s16x8 kf[4], vf[4], kt[8];
+  keep<64>(a,
+           reinterpret_cast<const char*>(a.k.p) +
+               2 * (s.batch * a.k.sb + s.kvh * a.k.sh + key * a.k.ss),
+           valid, lane, kf);
+  keep<64>(a,
+           reinterpret_cast<const char*>(a.v.p) +
+               2 * (s.batch * a.v.sb + s.kvh * a.v.sh + key * a.v.ss),
+           valid, lane, vf);
+  // D of all rows: 4 elements a thread, 16 threads a row
+  {
+    int de = (threadIdx.x & 15) * 4;
+    const T* ob = reinterpret_cast<const T*>(a.out) +
+                  (((long)s.batch * a.sq) * a.hk * a.g + (long)s.kvh * a.g) *
+                      a.hd +
+                  de;
+    const T* db = reinterpret_cast<const T*>(din.base) + de;
+    uint2 ov[8], dv[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      int r = i * 32 + (threadIdx.x >> 4);
+      ov[i] = dv[i] = {0, 0};
+      if (r < s.rows && de < a.hd) {
+        int pos = (int)mdiv(r, a.g_mul, a.g_shift), hd = r - pos * a.g;
+        ov[i] = *reinterpret_cast<const uint2*>(
+            ob + ((long)pos * a.hk * a.g + hd) * a.hd);
+        dv[i] = *reinterpret_cast<const uint2*>(db + pos * a.dout.ss +
+                                                hd * a.dout.sh);
+      }
+    }
+    if (threadIdx.x < 256)
+      lse[threadIdx.x] =
+          threadIdx.x < s.rows
+              ? a.lse[(long)bh * a.sq * a.g + threadIdx.x]
+              : INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const T* x = reinterpret_cast<const T*>(&ov[i]);
+      const T* y = reinterpret_cast<const T*>(&dv[i]);
+      float d = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d += to_f32(x[j]) * to_f32(y[j]);
+#pragma unroll
+      for (int m = 1; m < 16; m <<= 1) d += __shfl_xor(d, m, 64);
+      if ((threadIdx.x & 15) == 0) del[i * 32 + (threadIdx.x >> 4)] = d;
+    }
+  }
+  staged();
+  // the wave's piece of dQ: d = 16*dg.., rows 16*rg..; its K^T operand
+  int dg = wave >> 1, rg = wave & 1, l4 = (lane & 15) >> 2, seg = lane & 3;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    int row = k * 32 + (lane >> 4) * 8 + l4;
+    int chunk = dg * 2 + (seg >> 1);
+    const char* x = ds01 + (seg & 1) * 8;
+    kt[k] = read_tr2(x + lds_at<64>(row, chunk),
+                     x + lds_at<64>(row + 4, chunk));
+  }
+  __syncthreads();  // K is read: the buffer is dS's
+  float c = a.scale * kLog2e;
+  f32x16 dk[2] = {kNone, kNone}, dv[2] = {kNone, kNone};
+  int nk = (s.klen + 31) / 32;
+
+  auto step = [&](int t, char* dso) {
+    if (!live) return;
+    const char* qt = qall + Geo<64>::bytes(32) * t;
+    const char* dt = dall + Geo<64>::bytes(32) * t;
+    const float *ls = lse + t * 32, *dl = del + t * 32;
+    f32x16 sc = kNone, dp = kNone;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      sc = Op<T>::mfma(frag_row<64>(qt, 0, ks, lane), kf[ks], sc);
+      dp = Op<T>::mfma(frag_row<64>(dt, 0, ks, lane), vf[ks], dp);
+    }
+    if (cut)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[i] = valid ? sc[i] : -INFINITY;
+    unsigned p[8], d[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float4 l4 = *reinterpret_cast<const float4*>(ls + j * 8 + h * 4);
+      float4 d4 = *reinterpret_cast<const float4*>(dl + j * 8 + h * 4);
+      const float *lp = &l4.x, *dd = &d4.x;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x = __builtin_amdgcn_exp2f(
+            fmaf(sc[4 * j + 2 * i], c, -lp[2 * i]));
+        float y = __builtin_amdgcn_exp2f(
+            fmaf(sc[4 * j + 2 * i + 1], c, -lp[2 * i + 1]));
+        p[2 * j + i] = Op<T>::pack(x, y);
+        d[2 * j + i] =
+            Op<T>::pack(x * (dp[4 * j + 2 * i] - dd[2 * i]),
+                        y * (dp[4 * j + 2 * i + 1] - dd[2 * i + 1]));
+      }
+      uint2 v = {d[2 * j], d[2 * j + 1]};
+      *reinterpret_cast<uint2*>(dso + key * 64 + ((j ^ perm2(key)) << 4) +
+                                ((h ^ ((key >> 3) & 1)) << 3)) = v;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        dv[i] = Op<T>::mfma(frag_col<64>(dt, k * 16, i, lane),
+                            pack8(p + 4 * k), dv[i]);
+        dk[i] = Op<T>::mfma(frag_col<64>(qt, k * 16, i, lane),
+                            pack8(d + 4 * k), dk[i]);
+      }
+  };
+  auto put_dq = [&](int t, const char* dso) {
+    f32x4v acc = {0.f, 0.f, 0.f, 0.f};
+    int j = 2 * rg + (seg >> 1);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k >= nk) break;
+      int x = k * 32 + (lane >> 4) * 8 + l4, y = x + 4;
+      acc = mfma16<T>(
+          kt[k],
+          read_tr2(dso + x * 64 + ((j ^ perm2(x)) << 4) +
+                       (((seg & 1) ^ ((x >> 3) & 1)) << 3),
+                   dso + y * 64 + ((j ^ perm2(y)) << 4) +
+                       (((seg & 1) ^ ((y >> 3) & 1)) << 3)),
+          acc);
+    }
+    int r = t * 32 + rg * 16 + (lane & 15), e = dg * 16 + (lane >> 4) * 4;
+    int pos = (int)mdiv(r, a.g_mul, a.g_shift);
+    if (pos < a.sq && e < a.hd) {
+      uint2 v = {Op<T>::pack(acc[0] * a.scale, acc[1] * a.scale),
+                 Op<T>::pack(acc[2] * a.scale, acc[3] * a.scale)};
+      *reinterpret_cast<uint2*>(
+          reinterpret_cast<T*>(a.dq) +
+          (((long)s.batch * a.sq + pos) * a.hk * a.g + s.kvh * a.g + r -
+           pos * a.g) *
+              a.hd +
+          e) = v;
+    }
+  };
+  // one barrier a step: a step's dS is read after it, while the next step
+  // fills the other half
+  for (int t = 0; t < ntile; ++t) {
+    char* dso = ds01 + (t & 1) * 256 * 64;
+    step(t, dso);
+    __syncthreads();
+    put_dq(t, dso);
+  }
+  if (key >= a.sk) return;
+  long at = (((long)s.batch * a.sk + key) * a.hk + s.kvh) * a.hd;
+  put_row<T, 2>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, a.hd, lane);
+  put_row<T, 2>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, a.hd, lane);
+}
+
 // x, y = sums over the splits of part[split][x then y], x times `scale`;
 // 4 elements a thread; nx and ny are multiples of 4
 template <typename T>
@@ -943,8 +1174,14 @@ struct Plan {
   int fwd, per;  // forward: parts over the keys, tiles of each
   bool few;      // rows fit one wave: attn_rc_few_k, tiles of 32
   int dq, dkv;   // backward: parts over the keys, over the rows
-  Plan(long b, long sq, long sk, long hk, long g) {
+  bool whole;    // backward in one pass: attn_rc_bwd_short_k
+  // free: no causal mask and no lengths
+  Plan(long b, long sq, long sk, long hk, long g, long hd, bool free) {
     long bh = b * hk, rows = sq * g;
+    // one block a head has to fill the chip. Sequences of few keys take D
+    // from P and dP, which only the two-pass backward does.
+    whole = free && hd <= 64 && sk > 64 && sk <= 256 && rows <= 256 &&
+            bh >= 256;
     long rblk = bh * ((rows + 127) / 128), kblk = bh * ((sk + 127) / 128);
     fwd = dq = dkv = 1;
     per = 0;
@@ -979,7 +1216,8 @@ template <typename T, int HDT>
 void launch(const Args& a, int bwd, float* ws, hipStream_t s) {
   int rblk = (a.sq * a.g + 127) / 128, kblk = (a.sk + 127) / 128;
   int bh = a.b * a.hk;
-  Plan p(a.b, a.sq, a.sk, a.hk, a.g);
+  Plan p(a.b, a.sq, a.sk, a.hk, a.g, a.hd,
+         !a.causal && !a.q_lens && !a.kv_lens);
   if (!bwd) {
     if (rblk == 0) return;
     if (p.few)
@@ -994,6 +1232,11 @@ void launch(const Args& a, int bwd, float* ws, hipStream_t s) {
     }
     return;
   }
+  if constexpr (HDT == 64)
+    if (p.whole) {
+      attn_rc_bwd_short_k<T><<<bh, 512, 0, s>>>(a);
+      return;
+    }
   long nq = (long)a.b * a.sq * a.hk * a.g * a.hd;
   long nk = (long)a.b * a.sk * a.hk * a.hd;
   if (rblk) {
@@ -1018,7 +1261,7 @@ extern "C" {
 // floats of workspace that forward or backward needs
 long pdta_attn_recompute_ws(long b, long sq, long sk, long hk, long g,
                             long hd, int bwd) {
-  Plan p(b, sq, sk, hk, g);
+  Plan p(b, sq, sk, hk, g, hd, false);
   long nq = b * sq * hk * g * hd, nk = b * sk * hk * hd;
   if (!bwd) return p.fwd > 1 ? p.fwd * (nq + nq / hd) : 0;
   long x = p.dq > 1 ? p.dq * nq : 0, y = p.dkv > 1 ? 2 * p.dkv * nk : 0;

@@ -138,6 +138,11 @@ CASES = [
     (1, 700, 1100, 2, 1, 64, True, None, None),
     (1, 1025, 1025, 4, 2, 128, True, None, None),
     (3, 5, 2000, 2, 1, 128, True, None, [2000, 3, 777]),
+    # many heads of 65 to 256 keys: backward in one pass
+    (64, 197, 197, 4, 4, 64, False, None, None),
+    (128, 70, 130, 6, 2, 40, False, None, None),
+    (256, 33, 256, 1, 1, 64, False, None, None),
+    (300, 1, 65, 3, 1, 8, False, None, None),
     # few rows against many keys, which are dealt out and joined
     (2, 1, 1000, 3, 3, 64, False, None, [0, 999]),
     (4, 3, 900, 6, 2, 96, True, [3, 0, 2, 1], [900, 5, 0, 513]),

@@ -4,6 +4,7 @@
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 
 #include <hip/hip_runtime_api.h>
 
@@ -394,6 +395,118 @@ std::vector<at::Tensor> attn_recompute_bwd(
   return {dq, dk, dv};
 }
 
+// ---- autograd -----------------------------------------------------------
+// The GPU path's autograd nodes are C++: the engine's device thread then runs
+// backward without taking the GIL, which for short sequences cost more than
+// the kernels (4 x 65 tokens of 3 heads, forward and backward: see the .hip
+// files).
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+c10::optional<at::Tensor> maybe(const at::Tensor& t) {
+  return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt;
+}
+at::Tensor plain(const c10::optional<at::Tensor>& t) {
+  return t.has_value() ? *t : at::Tensor();
+}
+void once(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what,
+              ": a gradient of the gradient is not supported");
+}
+
+// t itself if 16-byte accesses can walk its rows
+at::Tensor walkable(const at::Tensor& t) {
+  return t.dim() == 4 && t.stride(3) == 1 && rows8(t) ? t : t.contiguous();
+}
+
+struct AttentionRecompute
+    : public torch::autograd::Function<AttentionRecompute> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q0,
+                            const at::Tensor& k0, const at::Tensor& v0,
+                            const c10::optional<at::Tensor>& q_lens,
+                            const c10::optional<at::Tensor>& kv_lens,
+                            double scale, bool causal) {
+    at::Tensor q = walkable(q0), k = walkable(k0), v = walkable(v0);
+    auto r = attn_recompute_fwd(q, k, v, q_lens, kv_lens, scale, causal,
+                                true);
+    ctx->save_for_backward(
+        {q, k, v, r[0], r[1], plain(q_lens), plain(kv_lens)});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["causal"] = causal;
+    return r[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("attention_recompute");
+    auto s = ctx->get_saved_variables();
+    auto r = attn_recompute_bwd(s[0], s[1], s[2], s[3], s[4], walkable(g[0]),
+                                maybe(s[5]), maybe(s[6]),
+                                ctx->saved_data["scale"].toDouble(),
+                                ctx->saved_data["causal"].toBool());
+    return {r[0], r[1], r[2], at::Tensor(), at::Tensor(), at::Tensor(),
+            at::Tensor()};
+  }
+};
+
+at::Tensor attention_recompute(at::Tensor q, at::Tensor k, at::Tensor v,
+                               c10::optional<at::Tensor> q_lens,
+                               c10::optional<at::Tensor> kv_lens,
+                               double scale, bool causal) {
+  if (at::GradMode::is_enabled() &&
+      (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    return AttentionRecompute::apply(q, k, v, q_lens, kv_lens, scale, causal);
+  return attn_recompute_fwd(walkable(q), walkable(k), walkable(v), q_lens,
+                            kv_lens, scale, causal, false)[0];
+}
+
+at::Tensor inner1(const at::Tensor& t) {
+  return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+
+struct QKNormRope : public torch::autograd::Function<QKNormRope> {
+  using Opt = c10::optional<at::Tensor>;
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q0,
+                               const at::Tensor& k0, const Opt& wq,
+                               const Opt& wk, const Opt& cos, const Opt& sin,
+                               const Opt& pos, double eps,
+                               bool interleaved) {
+    at::Tensor q = inner1(q0), k = inner1(k0);
+    auto r = qk_norm_rope(q, k, wq, wk, cos, sin, pos, eps, interleaved,
+                          c10::nullopt, c10::nullopt);
+    ctx->save_for_backward(
+        {q, k, plain(wq), plain(wk), plain(cos), plain(sin), plain(pos)});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    return r;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("qk_norm_rope");
+    auto s = ctx->get_saved_variables();
+    for (int i = 0; i < 2; ++i)
+      if (!g[i].defined()) g[i] = at::zeros_like(s[i]);
+    auto r = qk_norm_rope(s[0], s[1], maybe(s[2]), maybe(s[3]), maybe(s[4]),
+                          maybe(s[5]), maybe(s[6]),
+                          ctx->saved_data["eps"].toDouble(),
+                          ctx->saved_data["interleaved"].toBool(),
+                          inner1(g[0]), inner1(g[1]));
+    r.resize(9);
+    return r;
+  }
+};
+
+std::vector<at::Tensor> qk_norm_rope_grad(
+    at::Tensor q, at::Tensor k, c10::optional<at::Tensor> wq,
+    c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cos,
+    c10::optional<at::Tensor> sin, c10::optional<at::Tensor> pos, double eps,
+    bool interleaved) {
+  bool w = wq.has_value() && wk.has_value() &&
+           (wq->requires_grad() || wk->requires_grad());
+  if (at::GradMode::is_enabled() &&
+      (q.requires_grad() || k.requires_grad() || w))
+    return QKNormRope::apply(q, k, wq, wk, cos, sin, pos, eps, interleaved);
+  return qk_norm_rope(inner1(q), inner1(k), wq, wk, cos, sin, pos, eps,
+                      interleaved, c10::nullopt, c10::nullopt);
+}
+
 }  // namespace
 
 void bind_transformer(pybind11::module_& m) {
@@ -414,4 +527,13 @@ void bind_transformer(pybind11::module_& m) {
         py::arg("k"), py::arg("v"), py::arg("out"), py::arg("lse"),
         py::arg("dout"), py::arg("q_lens"), py::arg("kv_lens"),
         py::arg("scale"), py::arg("causal"));
+  // differentiable forms
+  m.def("attention_recompute", &attention_recompute, py::arg("q"),
+        py::arg("k"), py::arg("v"), py::arg("q_lens"), py::arg("kv_lens"),
+        py::arg("scale"), py::arg("causal"),
+        py::call_guard<py::gil_scoped_release>());
+  m.def("qk_norm_rope_grad", &qk_norm_rope_grad, py::arg("q"), py::arg("k"),
+        py::arg("q_weight"), py::arg("k_weight"), py::arg("cos"),
+        py::arg("sin"), py::arg("positions"), py::arg("eps"),
+        py::arg("interleaved"), py::call_guard<py::gil_scoped_release>());
 }

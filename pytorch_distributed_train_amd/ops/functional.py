@@ -897,14 +897,6 @@ def attention_qkv(qkv2d, b, s, h, hd, nvalid, scale):
 # Attention with recomputed probabilities
 # ---------------------------------------------------------------------------
 
-def _rows8(x):
-    """x [b, s, h, hd] itself if 16-byte accesses can walk its rows."""
-    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(
-            x.shape[d] <= 1 or x.stride(d) % 8 == 0 for d in range(3)):
-        return x
-    return x.contiguous()
-
-
 def _visible(q, k, causal, q_lens, kv_lens):
     """[b, 1, 1, sq, sk] where a query may see a key, for the CPU path."""
     sq, sk = q.shape[1], k.shape[1]
@@ -921,16 +913,11 @@ def _visible(q, k, causal, q_lens, kv_lens):
 
 
 class AttentionRecomputeFn(torch.autograd.Function):
+    """CPU reference; the GPU path's node is C++ (bind_transformer.cpp)."""
+
     @staticmethod
     def forward(ctx, q, k, v, scale, causal, q_lens, kv_lens):
         ctx.scale, ctx.causal = scale, causal
-        if q.is_cuda:
-            q, k, v = _rows8(q), _rows8(k), _rows8(v)
-            out, lse = ext().attn_recompute_fwd(
-                q, k, v, q_lens, kv_lens, scale, causal,
-                any(ctx.needs_input_grad))
-            ctx.save_for_backward(q, k, v, out, lse, q_lens, kv_lens)
-            return out
         b, sq, h, hd = q.shape
         hk = k.shape[2]
         ok = _visible(q, k, causal, q_lens, kv_lens)
@@ -951,11 +938,6 @@ class AttentionRecomputeFn(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, out, lse, q_lens, kv_lens = ctx.saved_tensors
         scale, causal = ctx.scale, ctx.causal
-        if q.is_cuda:
-            dq, dk, dv = ext().attn_recompute_bwd(
-                q, k, v, out, lse, _rows8(dout), q_lens, kv_lens, scale,
-                causal)
-            return dq, dk, dv, None, None, None, None
         h, hk = q.shape[2], k.shape[2]
         ok = _visible(q, k, causal, q_lens, kv_lens)
         seen_k = ok.any(3)[:, 0, 0, :, None, None]
@@ -1032,6 +1014,9 @@ def attention_recompute(q, k, v, scale: float | None = None,
         q_lens, kv_lens = q_lens.long(), kv_lens.long()
     q_lens, kv_lens = (x if x is None else x.contiguous()
                        for x in (q_lens, kv_lens))
+    if q.is_cuda:
+        return ext().attention_recompute(q, k, v, q_lens, kv_lens, scale,
+                                         causal)
     return AttentionRecomputeFn.apply(q, k, v, float(scale), bool(causal),
                                       q_lens, kv_lens)
 
@@ -1091,6 +1076,9 @@ def _inner1(x):
 
 
 class QKNormRopeFn(torch.autograd.Function):
+    """CPU reference, and the GPU path with direct gradient slots (without
+    them its node is C++, bind_transformer.cpp)."""
+
     @staticmethod
     def forward(ctx, q, k, wq, wk, cos, sin, positions, eps, interleaved,
                 gslot_q, gslot_k):
@@ -1200,6 +1188,10 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None,
         raise ValueError(f"positions must be int32 or int64 [{b}, {s}]")
     if positions is not None:
         positions = positions.contiguous()
+    if q.is_cuda and gslot_q is None and gslot_k is None:
+        return tuple(ext().qk_norm_rope_grad(q, k, q_weight, k_weight, cos,
+                                             sin, positions, eps,
+                                             interleaved))
     return QKNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions,
                               eps, interleaved, gslot_q, gslot_k)
 

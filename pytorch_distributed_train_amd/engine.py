@@ -51,7 +51,9 @@ class Trainer:
         torch.manual_seed(args.seed)  # same init on all ranks (+ broadcast)
 
         num_classes = 10 if args.data == "synthetic-cifar10" else 1000
-        self.model = build_model(args.model, num_classes, self.compute_dtype)
+        self.model = build_model(
+            args.model, num_classes, self.compute_dtype,
+            qk_norm_rope=getattr(args, "qk_norm_rope", False))
         self.model.to(self.device)
 
         self.comm = make_communicator(self.env, self.device, args.backend)
@@ -163,6 +165,9 @@ class Trainer:
             elif isinstance(m, MultiheadSelfAttention):
                 m._gslot_inw = slot(m.in_proj_weight)
                 m._gslot_inb = slot(m.in_proj_bias)
+                if m.qk_norm_rope:
+                    m._gslot_qn = slot(m.q_norm_weight)
+                    m._gslot_kn = slot(m.k_norm_weight)
 
     def _flatten_nbt(self):
         from .models.layers import BatchNorm2dNHWC

@@ -26,6 +26,10 @@ def build_parser() -> argparse.ArgumentParser:
                    dest="local_rank",
                    help="set by the legacy launcher; prefer LOCAL_RANK env")
     p.add_argument("--model", default="resnet50", choices=MODEL_CHOICES)
+    p.add_argument("--qk-norm-rope", action="store_true",
+                   help="transformers: norm and rotate each head's queries "
+                        "and keys; attention recomputes its probabilities "
+                        "in backward")
     p.add_argument("--batch-size", type=int, default=256,
                    help="per-process (per-GPU) batch size")
     p.add_argument("--epochs", type=int, default=1)

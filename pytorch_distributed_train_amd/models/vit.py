@@ -11,9 +11,15 @@ of 64 — padded rows never mix into real rows (softmax masks key columns
 >= 197, padded V rows are zero, LN/MLP are row-local), so results for the
 class token are exact. Attention runs as batched MFMA GEMMs (QK^T in
 fp32) + a fused masked-softmax kernel (csrc/ln.hip).
+
+qk_norm_rope=True norms each head's queries and keys, turns them by the
+patch's row and column, and takes attention with recomputed probabilities
+(csrc/qknorm.hip, csrc/attn_recompute.hip); it adds two [head_dim] weights a
+layer to the state dict.
 """
 from __future__ import annotations
 
+import math
 from collections import OrderedDict
 
 import torch
@@ -60,14 +66,33 @@ class MultiheadSelfAttention(nn.Module):
     """torchvision-compatible parameter layout: in_proj_weight [3d, d],
     in_proj_bias [3d], out_proj Linear."""
 
-    def __init__(self, dim: int, num_heads: int):
+    def __init__(self, dim: int, num_heads: int,
+                 qk_norm_rope: bool = False):
         super().__init__()
         self.num_heads = num_heads
         self.head_dim = dim // num_heads
+        self.qk_norm_rope = qk_norm_rope
+        if qk_norm_rope:
+            self.q_norm_weight = nn.Parameter(torch.ones(self.head_dim))
+            self.k_norm_weight = nn.Parameter(torch.ones(self.head_dim))
+            self._rope = None
         self.in_proj_weight = nn.Parameter(torch.empty(3 * dim, dim))
         self.in_proj_bias = nn.Parameter(torch.zeros(3 * dim))
         nn.init.xavier_uniform_(self.in_proj_weight)
         self.out_proj = Linear(dim, dim)
+
+    def _tables(self, s: int, device):
+        """Rotation of a class token and a square grid of patches; not a
+        buffer, so that no checkpoint or broadcast carries it."""
+        if self._rope is None or self._rope[0].shape[0] != s \
+                or self._rope[0].device != device:
+            side = math.isqrt(s - 1)
+            if side * side != s - 1:
+                raise ValueError(f"{s} tokens are no class token and square "
+                                 "grid")
+            self._rope = OF.rope_tables_2d(side, side, self.head_dim,
+                                           prefix=1, device=device)
+        return self._rope
 
     def forward(self, x, nvalid: int | None = None):
         # x [B, s, d] — the encoder runs PACKED (s = 197): only this
@@ -91,6 +116,18 @@ class MultiheadSelfAttention(nn.Module):
                         gslot_b=(getattr(self, "_gslot_inb", None)
                                  if on_direct else None))
         scale = 1.0 / (hd ** 0.5)
+        if self.qk_norm_rope:
+            if nvalid != s:
+                raise ValueError("qk_norm_rope takes whole sequences")
+            cos, sin = self._tables(s, x.device)
+            out = OF.attention_qkv_rope(
+                qkv, self.q_norm_weight, self.k_norm_weight, cos, sin, b, s,
+                h, hd, scale,
+                gslot_q=(getattr(self, "_gslot_qn", None)
+                         if on_direct else None),
+                gslot_k=(getattr(self, "_gslot_kn", None)
+                         if on_direct else None))
+            return self.out_proj(out.reshape(b * s, d)).view(b, s, d)
         if x.is_cuda:
             # zero-copy path: q/k/v read in place, grads scattered in
             # place. The fused kernel consumes the PACKED [b, s=197, 3d]
@@ -126,10 +163,12 @@ class GELU(nn.Module):
 
 
 class EncoderBlock(nn.Module):
-    def __init__(self, dim: int, num_heads: int, mlp_dim: int):
+    def __init__(self, dim: int, num_heads: int, mlp_dim: int,
+                 qk_norm_rope: bool = False):
         super().__init__()
         self.ln_1 = LayerNorm(dim)
-        self.self_attention = MultiheadSelfAttention(dim, num_heads)
+        self.self_attention = MultiheadSelfAttention(dim, num_heads,
+                                                     qk_norm_rope)
         self.ln_2 = LayerNorm(dim)
         self.mlp = nn.Sequential(
             Linear(dim, mlp_dim), GELU(), nn.Identity(), Linear(mlp_dim, dim))
@@ -150,14 +189,15 @@ class EncoderBlock(nn.Module):
 
 class Encoder(nn.Module):
     def __init__(self, num_layers: int, dim: int, num_heads: int,
-                 mlp_dim: int):
+                 mlp_dim: int, qk_norm_rope: bool = False):
         super().__init__()
         self.pos_embedding = nn.Parameter(
             torch.empty(1, SEQ, dim).normal_(std=0.02))
         layers = OrderedDict()
         for i in range(num_layers):
             layers[f"encoder_layer_{i}"] = EncoderBlock(dim, num_heads,
-                                                        mlp_dim)
+                                                        mlp_dim,
+                                                        qk_norm_rope)
         self.layers = nn.Sequential(layers)
         self.ln = LayerNorm(dim)
 
@@ -171,7 +211,8 @@ class Encoder(nn.Module):
 class VisionTransformer(nn.Module):
     def __init__(self, image_size=224, patch_size=16, num_layers=12,
                  num_heads=12, hidden_dim=768, mlp_dim=3072,
-                 num_classes=1000, compute_dtype=None):
+                 num_classes=1000, compute_dtype=None,
+                 qk_norm_rope=False):
         super().__init__()
         self.compute_dtype = compute_dtype or torch.float32
         self.patch_size = patch_size
@@ -179,7 +220,8 @@ class VisionTransformer(nn.Module):
         self.class_token = nn.Parameter(torch.zeros(1, 1, hidden_dim))
         self.conv_proj = Conv2dNHWC(3, hidden_dim, patch_size,
                                     stride=patch_size, padding=0, bias=True)
-        self.encoder = Encoder(num_layers, hidden_dim, num_heads, mlp_dim)
+        self.encoder = Encoder(num_layers, hidden_dim, num_heads, mlp_dim,
+                               qk_norm_rope)
         self.heads = nn.Sequential(OrderedDict(
             [("head", Linear(hidden_dim, num_classes))]))
         nn.init.zeros_(self.heads.head.weight)
@@ -196,6 +238,7 @@ class VisionTransformer(nn.Module):
         return self.heads(x[:, 0].contiguous())    # class token -> logits
 
 
-def vit_b_16(num_classes=1000, compute_dtype=None):
+def vit_b_16(num_classes=1000, compute_dtype=None, qk_norm_rope=False):
     return VisionTransformer(num_classes=num_classes,
-                             compute_dtype=compute_dtype)
+                             compute_dtype=compute_dtype,
+                             qk_norm_rope=qk_norm_rope)

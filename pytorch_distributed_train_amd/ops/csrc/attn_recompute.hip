@@ -84,6 +84,7 @@ struct View {  // [b, s, heads, hd] of a 16-bit type, strides in elements
 struct Args {
   View q, k, v, dout;
   void *out, *dq, *dk, *dv;    // contiguous; out is read by backward
+  long vb, vs, vh;             // but dv has strides of its own
   float *lse, *delta;          // [b, hk, sq*g]; lse in base 2 of scaled scores
   const void *q_lens, *kv_lens;  // [b] int32 / int64, or null
   int lens64;
@@ -941,7 +942,9 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
     for (int i = 0; i < G::DT; ++i) dk[i] = dv[i] = kNone;
   long at = (((long)s.batch * a.sk + key) * a.hk + s.kvh) * a.hd;
   if (nsplit == 1) {
-    put_row<T, G::DT>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, a.hd, lane);
+    put_row<T, G::DT>(reinterpret_cast<T*>(a.dv) + s.batch * a.vb +
+                          key * a.vs + s.kvh * a.vh,
+                      dv, 1.f, a.hd, lane);
     put_row<T, G::DT>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, a.hd,
                       lane);
     return;
@@ -1144,16 +1147,18 @@ __global__ __launch_bounds__(512, 2) void attn_rc_bwd_short_k(Args a) {
   }
   if (key >= a.sk) return;
   long at = (((long)s.batch * a.sk + key) * a.hk + s.kvh) * a.hd;
-  put_row<T, 2>(reinterpret_cast<T*>(a.dv) + at, dv, 1.f, a.hd, lane);
+  put_row<T, 2>(reinterpret_cast<T*>(a.dv) + s.batch * a.vb + key * a.vs +
+                    s.kvh * a.vh,
+                dv, 1.f, a.hd, lane);
   put_row<T, 2>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, a.hd, lane);
 }
 
-// x, y = sums over the splits of part[split][x then y], x times `scale`;
-// 4 elements a thread; nx and ny are multiples of 4
+// x = scale * sums over the splits of part[split][nx + ny], then dv the sums
+// of the ny behind; 4 elements a thread; nx and ny are multiples of 4
 template <typename T>
 __global__ __launch_bounds__(256) void attn_rc_join_k(
-    const float* __restrict__ part, long nx, long ny, int nsplit, float scale,
-    T* __restrict__ x, T* __restrict__ y) {
+    const float* __restrict__ part, long nx, long ny, int nsplit, T* x,
+    Args a) {
   long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= nx + ny) return;
   float4 sum = {0.f, 0.f, 0.f, 0.f};
@@ -1162,10 +1167,19 @@ __global__ __launch_bounds__(256) void attn_rc_join_k(
     float4 v = *reinterpret_cast<const float4*>(part + k * (nx + ny) + i);
     sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
   }
-  float m = i < nx ? scale : 1.f;
+  float m = i < nx ? a.scale : 1.f;
   uint2 v = {Op<T>::pack(sum.x * m, sum.y * m),
              Op<T>::pack(sum.z * m, sum.w * m)};
-  *reinterpret_cast<uint2*>(i < nx ? x + i : y + (i - nx)) = v;
+  T* to = x + i;
+  if (i >= nx) {
+    long row = (i - nx) / a.hd;
+    int d = (int)(i - nx - row * a.hd), kvh = (int)(row % a.hk);
+    row /= a.hk;
+    long batch = row / a.sk;
+    to = reinterpret_cast<T*>(a.dv) + batch * a.vb +
+         (row - batch * a.sk) * a.vs + kvh * a.vh + d;
+  }
+  *reinterpret_cast<uint2*>(to) = v;
 }
 
 // How work is dealt out where there are few blocks; shapes alone decide. Two
@@ -1243,14 +1257,14 @@ void launch(const Args& a, int bwd, float* ws, hipStream_t s) {
     attn_rc_dq_k<T, HDT><<<bh * rblk * p.dq, 256, 0, s>>>(a, rblk, p.dq, ws);
     if (p.dq > 1)
       attn_rc_join_k<T><<<(nq / 4 + 255) / 256, 256, 0, s>>>(
-          ws, nq, 0, p.dq, a.scale, (T*)a.dq, nullptr);
+          ws, nq, 0, p.dq, (T*)a.dq, a);
   }
   if (kblk) {
     attn_rc_dkv_k<T, HDT>
         <<<bh * kblk * p.dkv, 256, 0, s>>>(a, kblk, p.dkv, ws);
     if (p.dkv > 1)
       attn_rc_join_k<T><<<(nk / 2 + 255) / 256, 256, 0, s>>>(
-          ws, nk, nk, p.dkv, a.scale, (T*)a.dk, (T*)a.dv);
+          ws, nk, nk, p.dkv, (T*)a.dk, a);
   }
 }
 
@@ -1268,8 +1282,8 @@ long pdta_attn_recompute_ws(long b, long sq, long sk, long hk, long g,
   return x > y ? x : y;
 }
 
-// strides: q, k, v, dout, each (b, s, head) in elements; multiples of 8, all
-// pointers 16-byte aligned, hd a multiple of 8 up to 128. lens null or [b].
+// strides: q, k, v, dout, dv, each (b, s, head) in elements; multiples of 8,
+// all pointers 16-byte aligned, hd a multiple of 8 up to 128. lens null or [b].
 // Forward writes out and, unless null, lse; backward reads both and writes
 // delta, dq, dk, dv; either with pdta_attn_recompute_ws floats in ws. Grids must stay below 2^31 blocks and sq*g below 2^31.
 void pdta_attn_recompute(const void* q, const void* k, const void* v,
@@ -1292,6 +1306,7 @@ void pdta_attn_recompute(const void* q, const void* k, const void* v,
   a.v = view(v, st + 6, false);
   a.dout = view(dout, st + 9, true);
   a.out = out, a.dq = dq, a.dk = dk, a.dv = dv, a.lse = lse, a.delta = delta;
+  a.vb = st[12], a.vs = st[13], a.vh = st[14];
   a.q_lens = q_lens, a.kv_lens = kv_lens, a.lens64 = lens64;
   a.b = b, a.sq = sq, a.sk = sk, a.hk = hk, a.g = g, a.hd = hd;
   a.scale = scale, a.causal = causal;

@@ -17,7 +17,8 @@ void pdta_adamw(float*, const float*, void*, void*, float*, float*, long,
                 const unsigned char*, float, unsigned, void*, hipStream_t);
 int pdta_qknorm_rows(long, int, int);
 void pdta_qknorm(const void* const*, const long*, const void* const*,
-                 const long*, const float* const*, void* const*, const int*,
+                 const long*, const float* const*, void* const*, const long*,
+                 const int*,
                  const float*, const float*, const void*, int, int, int, int,
                  long, long, float, int, int, int, float*, float*, float*,
                  int, hipStream_t);
@@ -120,13 +121,15 @@ bool rows8(const at::Tensor& t) {
 }
 
 // dq, dk undefined: forward -> {q', k'}; else backward -> {dx_q, dx_k,
-// dw_q, dw_k} (the last two empty without weights)
+// dw_q, dw_k} (the last two empty without weights). outs: where the results
+// go instead of new tensors, in the same order.
+using Outs = std::vector<at::Tensor>;
 std::vector<at::Tensor> qk_norm_rope(
     at::Tensor q, at::Tensor k, c10::optional<at::Tensor> wq,
     c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cos,
     c10::optional<at::Tensor> sin, c10::optional<at::Tensor> positions,
     double eps, bool interleaved, c10::optional<at::Tensor> dq,
-    c10::optional<at::Tensor> dk) {
+    c10::optional<at::Tensor> dk, const Outs& outs = {}) {
   TORCH_CHECK(q.is_cuda(), "q must be on GPU");
   c10::DeviceGuard guard(q.device());
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) &&
@@ -213,35 +216,52 @@ std::vector<at::Tensor> qk_norm_rope(
     TORCH_CHECK(pos32 || positions->scalar_type() == at::kLong,
                 "positions must be int32 or int64");
   }
-  at::Tensor y[2];
+  at::Tensor y[2], dw[2];
   void* yp[2];
-  for (int i = 0; i < 2; ++i) {
-    y[i] = at::empty({b, s, heads[i], hd}, q.options());
-    yp[i] = y[i].data_ptr();
-  }
-  at::Tensor part, dwq, dwk;
+  long ys[6];
   auto f32 = q.options().dtype(at::kFloat);
-  if (bwd && norm) {
-    int rows = pdta_qknorm_rows(b * s, heads[0] + heads[1], vec);
-    if (rows == 0)
-      return {y[0], y[1], at::zeros({hd}, f32), at::zeros({hd}, f32)};
-    part = at::empty({rows, 2 * hd}, f32);
-    dwq = at::empty({hd}, f32);
-    dwk = at::empty({hd}, f32);
+  bool dws = bwd && norm;
+  TORCH_CHECK(outs.empty() || outs.size() == (dws ? 4 : 2),
+              "outs must be all results");
+  for (int i = 0; i < 2; ++i) {
+    if (outs.empty()) {
+      y[i] = at::empty({b, s, heads[i], hd}, q.options());
+      if (dws) dw[i] = at::empty({hd}, f32);
+    } else {
+      y[i] = outs[i];
+      TORCH_CHECK(y[i].device() == q.device() &&
+                      y[i].scalar_type() == q.scalar_type() &&
+                      y[i].sizes() == t[i].sizes() &&
+                      (y[i].numel() == 0 || y[i].stride(3) == 1),
+                  "a result must be like its input");
+      if (dws) {
+        dw[i] = outs[2 + i];
+        check_flat("a weight's gradient", dw[i], q, at::kFloat, hd);
+      }
+    }
+    vec = vec && rows8(y[i]);
+    yp[i] = y[i].data_ptr();
+    for (int j = 0; j < 3; ++j) ys[3 * i + j] = y[i].stride(j);
   }
-  pdta_qknorm(x, xs, dy, gs, w, yp, heads,
+  at::Tensor part;
+  if (dws) {
+    int rows = pdta_qknorm_rows(b * s, heads[0] + heads[1], vec);
+    if (rows == 0) return {y[0], y[1], dw[0].zero_(), dw[1].zero_()};
+    part = at::empty({rows, 2 * hd}, f32);
+  }
+  pdta_qknorm(x, xs, dy, gs, w, yp, ys, heads,
               rot ? cos->data_ptr<float>() : nullptr,
               rot ? sin->data_ptr<float>() : nullptr,
               positions.has_value() ? positions->data_ptr() : nullptr, pos32,
               npos, rot, hd, b, s, (float)eps, interleaved, vec, bwd,
-              bwd && norm ? part.data_ptr<float>() : nullptr,
-              bwd && norm ? dwq.data_ptr<float>() : nullptr,
-              bwd && norm ? dwk.data_ptr<float>() : nullptr, dt_of(q),
+              dws ? part.data_ptr<float>() : nullptr,
+              dws ? dw[0].data_ptr<float>() : nullptr,
+              dws ? dw[1].data_ptr<float>() : nullptr, dt_of(q),
               cur_stream());
   launched("qk_norm_rope");
   if (!bwd) return {y[0], y[1]};
   if (!norm) return {y[0], y[1], at::Tensor(), at::Tensor()};
-  return {y[0], y[1], dwq, dwk};
+  return {y[0], y[1], dw[0], dw[1]};
 }
 
 // ---- attention with recomputed probabilities -----------------------------
@@ -326,7 +346,7 @@ std::vector<at::Tensor> attn_recompute_fwd(
   auto out = at::empty({n.b, n.sq, n.h, n.hd}, q.options());
   auto lse = at::empty({want_lse ? n.b * n.hk * n.sq * g : 0},
                        q.options().dtype(at::kFloat));
-  long st[12] = {0};
+  long st[15] = {0};
   attn_strides(q, st);
   attn_strides(k, st + 3);
   attn_strides(v, st + 6);
@@ -348,11 +368,12 @@ std::vector<at::Tensor> attn_recompute_fwd(
   return {out, lse};
 }
 
-// {dq, dk, dv}, contiguous
+// {dq, dk, dv}, contiguous; dv_out: where dv goes instead, with strides
 std::vector<at::Tensor> attn_recompute_bwd(
     at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at::Tensor lse,
     at::Tensor dout, c10::optional<at::Tensor> q_lens,
-    c10::optional<at::Tensor> kv_lens, double scale, bool causal) {
+    c10::optional<at::Tensor> kv_lens, double scale, bool causal,
+    c10::optional<at::Tensor> dv_out = c10::nullopt) {
   TORCH_CHECK(q.is_cuda(), "q must be on GPU");
   c10::DeviceGuard guard(q.device());
   AttnShape n = attn_check(q, k, v, q_lens, kv_lens, scale);
@@ -371,16 +392,22 @@ std::vector<at::Tensor> attn_recompute_bwd(
               "lse must be the forward's");
   auto dq = at::empty({n.b, n.sq, n.h, n.hd}, q.options());
   auto dk = at::empty({n.b, n.sk, n.hk, n.hd}, q.options());
-  auto dv = at::empty_like(dk);
+  at::Tensor dv = dv_out.has_value() ? *dv_out : at::empty_like(dk);
+  TORCH_CHECK(dv.device() == q.device() &&
+                  dv.scalar_type() == q.scalar_type() &&
+                  dv.sizes() == dk.sizes() &&
+                  (dv.numel() == 0 || (dv.stride(3) == 1 && rows8(dv))),
+              "dv_out must be like v, with aligned rows");
   auto delta = at::empty_like(lse);
   auto ws = at::empty(
       {pdta_attn_recompute_ws(n.b, n.sq, n.sk, n.hk, g, n.hd, 1)},
       lse.options());
-  long st[12];
+  long st[15];
   attn_strides(q, st);
   attn_strides(k, st + 3);
   attn_strides(v, st + 6);
   attn_strides(dout, st + 9);
+  attn_strides(dv, st + 12);
   if (dq.numel() || dk.numel()) {
     pdta_attn_recompute(q.data_ptr(), k.data_ptr(), v.data_ptr(),
                         dout.data_ptr(), st, out.data_ptr(),
@@ -519,14 +546,15 @@ void bind_transformer(pybind11::module_& m) {
         py::arg("q_weight"), py::arg("k_weight"), py::arg("cos"),
         py::arg("sin"), py::arg("positions"), py::arg("eps"),
         py::arg("interleaved"), py::arg("dq") = py::none(),
-        py::arg("dk") = py::none());
+        py::arg("dk") = py::none(), py::arg("outs") = Outs());
   m.def("attn_recompute_fwd", &attn_recompute_fwd, py::arg("q"),
         py::arg("k"), py::arg("v"), py::arg("q_lens"), py::arg("kv_lens"),
         py::arg("scale"), py::arg("causal"), py::arg("want_lse"));
   m.def("attn_recompute_bwd", &attn_recompute_bwd, py::arg("q"),
         py::arg("k"), py::arg("v"), py::arg("out"), py::arg("lse"),
         py::arg("dout"), py::arg("q_lens"), py::arg("kv_lens"),
-        py::arg("scale"), py::arg("causal"));
+        py::arg("scale"), py::arg("causal"),
+        py::arg("dv_out") = py::none());
   // differentiable forms
   m.def("attention_recompute", &attention_recompute, py::arg("q"),
         py::arg("k"), py::arg("v"), py::arg("q_lens"), py::arg("kv_lens"),

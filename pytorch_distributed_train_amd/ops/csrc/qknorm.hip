@@ -25,7 +25,8 @@ struct HeadsIn {  // one tensor [b, s, heads, hd], strides in elements
   const void* dy;  // backward: gradient of y, same kind of strides
   long gb, gs, gh;
   const float* w;  // [hd] or null
-  void* y;         // contiguous [b, s, heads, hd]: y forward, dx backward
+  void* y;         // y forward, dx backward
+  long yb, ys, yh;
   int heads;
 };
 
@@ -170,8 +171,8 @@ __global__ __launch_bounds__(256) void qknorm_fwd_k(Args a) {
       Vec8<T> v;
 #pragma unroll
       for (int i = 0; i < 8; ++i) v.v[i] = from_f32<T>(x[i]);
-      store8(reinterpret_cast<T*>(t.y) + (tok * t.heads + head) * a.hd +
-                 chunk * 8,
+      store8(reinterpret_cast<T*>(t.y) + b * t.yb + srow * t.ys +
+                 head * t.yh + chunk * 8,
              v);
     }
   }
@@ -251,8 +252,8 @@ __global__ __launch_bounds__(256) void qknorm_bwd_k(Args a,
         Vec8<T> v;
 #pragma unroll
         for (int i = 0; i < 8; ++i) v.v[i] = from_f32<T>(g[i]);
-        store8(reinterpret_cast<T*>(t.y) + (tok * t.heads + head) * a.hd +
-                   chunk * 8,
+        store8(reinterpret_cast<T*>(t.y) + b * t.yb + srow * t.ys +
+                   head * t.yh + chunk * 8,
                v);
       }
     }
@@ -305,7 +306,7 @@ __global__ __launch_bounds__(256) void qknorm_any_k(Args a, int inter,
                   head * t.sh;
     const T* gp = reinterpret_cast<const T*>(t.dy) + b * t.gb + srow * t.gs +
                   head * t.gh;
-    T* yp = reinterpret_cast<T*>(t.y) + (tok * t.heads + head) * a.hd;
+    T* yp = reinterpret_cast<T*>(t.y) + b * t.yb + srow * t.ys + head * t.yh;
     int pos = a.rot ? position(a, tok, srow) : 0;
     float x[4], v[4], w[4], ss = 0.f;
 #pragma unroll
@@ -432,14 +433,14 @@ int pdta_qknorm_rows(long tokens, int nv, int vec) {
   return (int)(blocks < kBwdBlocks ? blocks : kBwdBlocks);
 }
 
-// Two tensors (queries, keys): x, dy pointers and element strides (b, s,
-// head), outputs contiguous. vec: hd a multiple of 8 up to 256, rot a
+// Two tensors (queries, keys): x, dy and y pointers and element strides (b,
+// s, head). vec: hd a multiple of 8 up to 256, rot a
 // multiple of 8 (16 for halves), strides multiples of 8 and all pointers
 // 16-byte aligned; else hd up to 256 and rot even. bwd: y is dx, part holds
 // pdta_qknorm_rows rows and dwq, dwk [hd] are written (norm only).
 void pdta_qknorm(const void* const* x, const long* xs, const void* const* dy,
                  const long* gs, const float* const* w, void* const* y,
-                 const int* heads, const float* cos, const float* sin,
+                 const long* ys, const int* heads, const float* cos, const float* sin,
                  const void* pos, int pos32, int npos, int rot, int hd,
                  long b, long s_len, float eps, int inter, int vec, int bwd,
                  float* part, float* dwq, float* dwk, int dt, hipStream_t s) {
@@ -447,7 +448,8 @@ void pdta_qknorm(const void* const* x, const long* xs, const void* const* dy,
   for (int k = 0; k < 2; ++k)
     a.t[k] = {x[k], xs[3 * k], xs[3 * k + 1], xs[3 * k + 2],
               dy[k], gs[3 * k], gs[3 * k + 1], gs[3 * k + 2],
-              w[k], y[k], heads[k]};
+              w[k], y[k], ys[3 * k], ys[3 * k + 1], ys[3 * k + 2],
+              heads[k]};
   a.cos = cos, a.sin = sin, a.pos = pos, a.pos32 = pos32, a.npos = npos;
   a.rot = rot, a.hd = hd, a.s = (int)s_len, a.tokens = b * s_len;
   a.eps = eps, a.slices = 1;

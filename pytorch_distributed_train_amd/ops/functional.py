@@ -965,7 +965,7 @@ def _heads_first(x, hk):
 
 def _heads_last(x, h):
     b, _, _, s, hd = x.shape
-    return x.permute(0, 3, 1, 2, 4).reshape(b, s, h, hd)
+    return x.permute(0, 3, 1, 2, 4).reshape(b, s, h, hd).contiguous()
 
 
 def attention_recompute(q, k, v, scale: float | None = None,
@@ -1040,6 +1040,25 @@ def rope_tables(n: int, rot_dim: int, theta: float = 10000.0,
     return a.cos().float(), a.sin().float()
 
 
+def rope_tables_2d(rows: int, cols: int, rot_dim: int, theta: float = 100.0,
+                   prefix: int = 0, device=None):
+    """(cos, sin), fp32 [prefix + rows*cols, rot_dim/2], for a grid of
+    patches in row order: half of the angles turn with the row, half with
+    the column. `prefix` tokens before the grid (a class token) do not
+    turn."""
+    if rot_dim % 4:
+        raise ValueError(f"rot_dim must be a multiple of 4: {rot_dim}")
+    r, c = (rope_tables(n, rot_dim // 2, theta, device=device)
+            for n in (rows, cols))
+    out = []
+    for x, y, still in zip(r, c, (1.0, 0.0)):
+        grid = torch.cat([x[:, None].expand(rows, cols, -1),
+                          y[None].expand(rows, cols, -1)], -1)
+        out.append(torch.cat([x.new_full((prefix, rot_dim // 2), still),
+                              grid.reshape(rows * cols, -1)]))
+    return tuple(out)
+
+
 def _wide(x):
     # the CPU reference computes in fp32; fp64 stays, for differences
     return x if x.dtype == torch.float64 else x.float()
@@ -1071,24 +1090,13 @@ def _gathered(cos, sin, positions, s):
                  for t in (cos, sin))
 
 
-def _inner1(x):
-    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
-
-
 class QKNormRopeFn(torch.autograd.Function):
-    """CPU reference, and the GPU path with direct gradient slots (without
-    them its node is C++, bind_transformer.cpp)."""
+    """CPU reference; the GPU path's node is C++ (bind_transformer.cpp)."""
 
     @staticmethod
-    def forward(ctx, q, k, wq, wk, cos, sin, positions, eps, interleaved,
-                gslot_q, gslot_k):
+    def forward(ctx, q, k, wq, wk, cos, sin, positions, eps, interleaved):
         ctx.eps, ctx.interleaved = eps, interleaved
-        ctx.gslot = (gslot_q, gslot_k)
         ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
-        if q.is_cuda:
-            return tuple(ext().qk_norm_rope(
-                _inner1(q), _inner1(k), wq, wk, cos, sin, positions, eps,
-                interleaved))
 
         def one(x, w):
             x32 = _wide(x)
@@ -1105,41 +1113,30 @@ class QKNormRopeFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq, dk):
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
-        if q.is_cuda:
-            dq, dk, dwq, dwk = ext().qk_norm_rope(
-                _inner1(q), _inner1(k), wq, wk, cos, sin, positions, ctx.eps,
-                ctx.interleaved, dq=_inner1(dq), dk=_inner1(dk))
-        else:
-            def one(x, w, dy):
-                g = _wide(dy)
-                if cos is not None:
-                    c, s = _gathered(cos, sin, positions, x.shape[1])
-                    g = _rotate(g, c, -s, ctx.interleaved)
-                if w is None:
-                    return g.to(x.dtype), None
-                x32 = _wide(x)
-                r = (x32.square().mean(-1, keepdim=True) + ctx.eps).rsqrt()
-                xhat = x32 * r
-                dw = (g * xhat).sum((0, 1, 2))
-                g = g * _wide(w)
-                dx = r * (g - xhat * (g * xhat).mean(-1, keepdim=True))
-                return dx.to(x.dtype), dw
 
-            dq, dwq = one(q, wq, dq)
-            dk, dwk = one(k, wk, dk)
-        dw = [dwq, dwk]
-        for i, slot in enumerate(ctx.gslot):
-            if slot is not None and dw[i] is not None:
-                slot[0].copy_(dw[i])
-                if slot[1] is not None:
-                    slot[1]()
-                dw[i] = None
-        return (dq, dk, *dw, None, None, None, None, None, None, None)
+        def one(x, w, dy):
+            g = _wide(dy)
+            if cos is not None:
+                c, s = _gathered(cos, sin, positions, x.shape[1])
+                g = _rotate(g, c, -s, ctx.interleaved)
+            if w is None:
+                return g.to(x.dtype), None
+            x32 = _wide(x)
+            r = (x32.square().mean(-1, keepdim=True) + ctx.eps).rsqrt()
+            xhat = x32 * r
+            dw = (g * xhat).sum((0, 1, 2))
+            g = g * _wide(w)
+            dx = r * (g - xhat * (g * xhat).mean(-1, keepdim=True))
+            return dx.to(x.dtype), dw
+
+        dq, dwq = one(q, wq, dq)
+        dk, dwk = one(k, wk, dk)
+        return dq, dk, dwq, dwk, None, None, None, None, None
 
 
 def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None,
-                 positions=None, eps: float = 1e-6, interleaved: bool = False,
-                 gslot_q=None, gslot_k=None):
+                 positions=None, eps: float = 1e-6,
+                 interleaved: bool = False):
     """RMS norm of every query and key head with the position rotation in
     the same pass: (q', k'), contiguous.
 
@@ -1188,12 +1185,76 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None,
         raise ValueError(f"positions must be int32 or int64 [{b}, {s}]")
     if positions is not None:
         positions = positions.contiguous()
-    if q.is_cuda and gslot_q is None and gslot_k is None:
+    if q.is_cuda:
         return tuple(ext().qk_norm_rope_grad(q, k, q_weight, k_weight, cos,
                                              sin, positions, eps,
                                              interleaved))
     return QKNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions,
-                              eps, interleaved, gslot_q, gslot_k)
+                              eps, interleaved)
+
+
+class AttentionQKVRopeFn(torch.autograd.Function):
+    """qk_norm_rope and attention_recompute over one projection's output
+    [b*s, 3*h*hd], as attention_qkv: q, k and v are read in place, and
+    backward writes its three parts of d(qkv) in place, so nothing is split,
+    stacked or copied. GPU only; the CPU path composes the two."""
+
+    @staticmethod
+    def forward(ctx, qkv2d, wq, wk, cos, sin, b, s, h, hd, scale, causal,
+                eps, gslot_q, gslot_k):
+        q, k, v = qkv2d.view(b, s, 3, h, hd).unbind(2)
+        qn, kn = ext().qk_norm_rope(q, k, wq, wk, cos, sin, None, eps, False)
+        out, lse = ext().attn_recompute_fwd(qn, kn, v, None, None, scale,
+                                            causal, True)
+        ctx.save_for_backward(qkv2d, wq, wk, cos, sin, qn, kn, out, lse)
+        ctx.dims = (b, s, h, hd, scale, causal, eps)
+        ctx.gslot = (gslot_q, gslot_k)
+        return out.view(b, s, h * hd)
+
+    @staticmethod
+    def backward(ctx, dout):
+        qkv2d, wq, wk, cos, sin, qn, kn, out, lse = ctx.saved_tensors
+        b, s, h, hd, scale, causal, eps = ctx.dims
+        q, k, v = qkv2d.view(b, s, 3, h, hd).unbind(2)
+        dqkv = torch.empty_like(qkv2d)
+        dq, dk, dv = dqkv.view(b, s, 3, h, hd).unbind(2)
+        dqn, dkn, _ = ext().attn_recompute_bwd(
+            qn, kn, v, out, lse, dout.contiguous().view(b, s, h, hd), None,
+            None, scale, causal, dv_out=dv)
+        dw = [torch.empty_like(w) if slot is None else slot[0]
+              for w, slot in zip((wq, wk), ctx.gslot)]
+        ext().qk_norm_rope(q, k, wq, wk, cos, sin, None, eps, False, dq=dqn,
+                           dk=dkn, outs=[dq, dk, *dw])
+        for i, slot in enumerate(ctx.gslot):
+            if slot is not None:
+                dw[i] = None
+                if slot[1] is not None:
+                    slot[1]()
+        return (dqkv, *dw) + (None,) * 11
+
+
+def attention_qkv_rope(qkv2d, q_weight, k_weight, cos, sin, b: int, s: int,
+                       h: int, hd: int, scale: float | None = None,
+                       causal: bool = False, eps: float = 1e-6,
+                       gslot_q=None, gslot_k=None):
+    """Multi-head attention over the interleaved projection [b*s, 3*h*hd]
+    with normed and rotated queries and keys (qk_norm_rope, halves layout)
+    and no s x s tensor (attention_recompute): [b, s, h*hd]. Gradients of
+    the projection come in its layout; of the weights directly into gslot_q,
+    gslot_k when given."""
+    if qkv2d.shape != (b * s, 3 * h * hd):
+        raise ValueError(f"qkv must be [{b * s}, {3 * h * hd}]: "
+                         f"{tuple(qkv2d.shape)}")
+    if scale is None:
+        scale = hd ** -0.5
+    if qkv2d.is_cuda:
+        return AttentionQKVRopeFn.apply(qkv2d.contiguous(), q_weight,
+                                        k_weight, cos, sin, b, s, h, hd,
+                                        scale, causal, eps, gslot_q, gslot_k)
+    q, k, v = qkv2d.view(b, s, 3, h, hd).unbind(2)
+    q, k = qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps=eps)
+    return attention_recompute(q, k, v, scale=scale, causal=causal) \
+        .view(b, s, h * hd)
 
 
 # ---------------------------------------------------------------------------

@@ -163,9 +163,10 @@ DEV_INLINE int lds_at(int row, int chunk) {
 // 16*ks + 8*(lane >> 5) + 0..7; r0 a multiple of 16
 template <int HDT>
 DEV_INLINE s16x8 frag_row(const char* lds, int r0, int ks, int lane) {
+  // chunk bit 1 is in no perm: it stays out of the lane's part
   return *reinterpret_cast<const s16x8*>(
-      lds + Geo<HDT>::bytes(r0) +
-      lds_at<HDT>(lane & 31, 2 * ks + (lane >> 5)));
+      lds + Geo<HDT>::bytes(r0) + (ks & 1) * 32 +
+      lds_at<HDT>(lane & 31, 2 * (ks & ~1) + (lane >> 5)));
 }
 
 DEV_INLINE s16x8 read_tr2(const char* lo, const char* hi) {
@@ -546,6 +547,44 @@ __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk,
     staged();
   }
   run.put(a, s, row, bh, nsplit, split, part, lane);
+}
+
+// ---- forward of short sequences: 256 keys at most, heads up to 64 ---------
+// All of K and V is loaded at once and 8 waves take 256 packed rows: a step is
+// shorter than a load's latency, which is paid once instead of once a tile.
+template <typename T>
+__global__ __launch_bounds__(512, 4) void attn_rc_fwd_short_k(Args a,
+                                                              int nblk) {
+  using G = Geo<64>;
+  LDS_BUFFER(kall, G::bytes(256));
+  LDS_BUFFER(vall, G::bytes(256));
+  int lane = threadIdx.x & 63;
+  int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int bh, blk;
+  place(a, nblk, true, &bh, &blk);
+  Seq s(a, bh);
+  Stream<64, 64, false, 8> kin(a, a.k, s, lane), vin(a, a.v, s, lane);
+  int end = blk * 256 < s.rows ? s.klen : 0;
+  int ntile = (end + 63) / 64;
+  for (int t = 0; t < ntile; ++t) {
+    kin.load(a, t * 64, s.klen, kall + G::bytes(64) * t, wave, lane);
+    vin.load(a, t * 64, s.klen, vall + G::bytes(64) * t, wave, lane);
+  }
+  Row row(a, s, blk * 256 + wave * 32 + (lane & 31));
+  s16x8 qf[4];
+  keep<64>(a,
+           reinterpret_cast<const char*>(a.q.p) +
+               2 * (s.batch * a.q.sb + row.pos * a.q.ss + row.head * a.q.sh),
+           row.valid, lane, qf);
+  int wlo = wave_min(row.lim), whi = wave_max(row.valid ? row.lim : 0);
+  Running<T, 64> run(a.scale);
+  staged();
+  for (int t = 0; t < ntile; ++t) {
+    if (t * 64 >= whi) break;
+    run.template step<2>(kall + G::bytes(64) * t, vall + G::bytes(64) * t, qf,
+                         t * 64, row.lim, wlo, lane);
+  }
+  run.put(a, s, row, bh, 1, 0, nullptr, lane);
 }
 
 // ---- forward of few rows (32 at most: single tokens) ----------------------
@@ -956,19 +995,23 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
 }
 
 // ---- backward of short sequences: all three gradients in one pass ---------
-// 65 to 256 keys, as many packed rows, heads up to 64: a block of 8 waves
-// holds a key head's keys, 32 a wave, and runs over its rows 32 at a time, so
-// S, dP and the exponentials are worked out once and q, k, v, out and dout
-// are read once, all at the start: a step is shorter than a load's latency.
-// dK and dV gather in registers as in attn_rc_dkv_k. dQ needs all keys of a
-// row: the waves put dS (16 bits, which it has as an operand anyway) to LDS,
-// and after the step's one barrier each takes a 16 x 16 piece of dQ over all
-// keys, K^T kept in registers. dS rows are one key's 32 rows, 64 bytes;
-// 8-byte piece (j, h) lies at (j ^ perm2(key), h ^ key bit 3): 16 keys'
-// writes and the transposing reads' 4 keys x 32 bytes meet distinct banks.
+// 65 to 256 keys, as many packed rows, heads up to 64: a block of 4 waves
+// holds a key head's keys, a wave one or two groups of 32, and runs over its
+// rows 32 at a time, so S, dP and the exponentials are worked out once, and
+// q, k, v, out and dout are read once. Two blocks share a CU, so that one's
+// loads and barriers pass under the other's products (one block of 8 waves
+// took 158 us at 1536 heads of 197 tokens). dK and dV gather in registers as
+// in attn_rc_dkv_k. dQ needs all keys of a row: the waves put dS (16 bits,
+// which it has as an operand anyway) to LDS, and after a barrier each takes 16 columns of dQ's 32 rows over all keys, in 16x16x32 products.
+// dS lies by key, 32 rows or 64 bytes each, with its 8-byte pieces moved
+// about (ds_at) so that 32 keys' writes and the transposing reads' 8 keys x
+// 32 bytes meet distinct banks.
 typedef float f32x4v __attribute__((ext_vector_type(4)));
-DEV_INLINE int perm2(int key) {
-  return (((key >> 1) & 1) << 1) | ((key >> 2) & 1);
+// row r (0..31, a multiple of 4) of a key's dS
+DEV_INLINE int ds_at(int key, int r) {
+  int f = ((key >> 2) & 2) | ((key >> 2) & 1);
+  return key * 64 + (((r >> 3) ^ f) << 4) +
+         ((((r >> 2) ^ (key >> 4)) & 1) << 3);
 }
 template <typename T> DEV_INLINE f32x4v mfma16(s16x8 a, s16x8 b, f32x4v c);
 template <>
@@ -982,175 +1025,209 @@ DEV_INLINE f32x4v mfma16<__half>(s16x8 a, s16x8 b, f32x4v c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(
       __builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-template <typename T>
-__global__ __launch_bounds__(512, 2) void attn_rc_bwd_short_k(Args a) {
-  LDS_BUFFER(qall, Geo<64>::bytes(256));
-  LDS_BUFFER(dall, Geo<64>::bytes(256));
-  LDS_BUFFER(ds01, Geo<64>::bytes(256));  // two steps' dS; first K, all of it
-  __shared__ float lse[256], del[256];
+
+// NKG: groups of 32 keys there is room for. (A second dS buffer in place of
+// the step's second barrier made no difference.)
+template <typename T, int NKG>
+__global__ __launch_bounds__(256, 2) void attn_rc_bwd_short_k(Args a) {
+  using G = Geo<64>;
+  constexpr int KG = (NKG + 3) / 4;  // groups of a wave: wave, wave + 4
+  LDS_BUFFER(kall, G::bytes(NKG * 32));
+  LDS_BUFFER(q0, G::bytes(32));
+  LDS_BUFFER(q1, G::bytes(32));
+  LDS_BUFFER(d0, G::bytes(32));
+  LDS_BUFFER(d1, G::bytes(32));
+  LDS_BUFFER(dso, NKG * 32 * 64);
+  __shared__ __attribute__((aligned(16))) float lse[256], del[256];
   int lane = threadIdx.x & 63, h = lane >> 5;
   int wave = uniform(threadIdx.x >> 6);
   int bh = blockIdx.x;
   Seq s(a, bh);
-  int key = wave * 32 + (lane & 31);
-  bool valid = key < s.klen;
-  bool cut = wave_max(!valid) != 0, live = wave * 32 < s.klen;
   int ntile = (s.rows + 31) / 32;
-  Stream<64, 256, false, 8> kin(a, a.k, s, lane);
-  Stream<64, 256, true, 8> qin(a, a.q, s, lane), din(a, a.dout, s, lane);
-  kin.load(a, 0, s.klen, ds01, wave, lane);
-  qin.load(a, 0, s.rows, qall, wave, lane);
-  din.load(a, 0, s.rows, dall, wave, lane);
-  s16x8 kf[4], vf[4], kt[8];
-  keep<64>(a,
-           reinterpret_cast<const char*>(a.k.p) +
-               2 * (s.batch * a.k.sb + s.kvh * a.k.sh + key * a.k.ss),
-           valid, lane, kf);
-  keep<64>(a,
-           reinterpret_cast<const char*>(a.v.p) +
-               2 * (s.batch * a.v.sb + s.kvh * a.v.sh + key * a.v.ss),
-           valid, lane, vf);
-  // D of all rows: 4 elements a thread, 16 threads a row
+  Stream<64, NKG * 32, false> kin(a, a.k, s, lane);
+  Stream<64, 32, true> qin(a, a.q, s, lane), din(a, a.dout, s, lane);
+  kin.load(a, 0, s.klen, kall, wave, lane);
+  auto load = [&](int t, char* qd, char* dd) {
+    qin.load(a, t * 32, s.rows, qd, wave, lane);
+    din.load(a, t * 32, s.rows, dd, wave, lane);
+  };
+  load(0, q0, d0);
+  // D of all rows: 8 elements a thread, 8 threads a row
   {
-    int de = (threadIdx.x & 15) * 4;
+    int de = (threadIdx.x & 7) * 8;
     const T* ob = reinterpret_cast<const T*>(a.out) +
                   (((long)s.batch * a.sq) * a.hk * a.g + (long)s.kvh * a.g) *
                       a.hd +
                   de;
     const T* db = reinterpret_cast<const T*>(din.base) + de;
-    uint2 ov[8], dv[8];
+    uint4 ov[8], dv[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      int r = i * 32 + (threadIdx.x >> 4);
-      ov[i] = dv[i] = {0, 0};
+      int r = i * 32 + (threadIdx.x >> 3);
+      ov[i] = dv[i] = {0, 0, 0, 0};
       if (r < s.rows && de < a.hd) {
         int pos = (int)mdiv(r, a.g_mul, a.g_shift), hd = r - pos * a.g;
-        ov[i] = *reinterpret_cast<const uint2*>(
+        ov[i] = *reinterpret_cast<const uint4*>(
             ob + ((long)pos * a.hk * a.g + hd) * a.hd);
-        dv[i] = *reinterpret_cast<const uint2*>(db + pos * a.dout.ss +
+        dv[i] = *reinterpret_cast<const uint4*>(db + pos * a.dout.ss +
                                                 hd * a.dout.sh);
       }
     }
-    if (threadIdx.x < 256)
-      lse[threadIdx.x] =
-          threadIdx.x < s.rows
-              ? a.lse[(long)bh * a.sq * a.g + threadIdx.x]
-              : INFINITY;
+    lse[threadIdx.x] = threadIdx.x < s.rows
+                           ? a.lse[(long)bh * a.sq * a.g + threadIdx.x]
+                           : INFINITY;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const T* x = reinterpret_cast<const T*>(&ov[i]);
       const T* y = reinterpret_cast<const T*>(&dv[i]);
       float d = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) d += to_f32(x[j]) * to_f32(y[j]);
+      for (int j = 0; j < 8; ++j) d += to_f32(x[j]) * to_f32(y[j]);
 #pragma unroll
-      for (int m = 1; m < 16; m <<= 1) d += __shfl_xor(d, m, 64);
-      if ((threadIdx.x & 15) == 0) del[i * 32 + (threadIdx.x >> 4)] = d;
+      for (int m = 1; m < 8; m <<= 1) d += __shfl_xor(d, m, 64);
+      if ((threadIdx.x & 7) == 0) del[i * 32 + (threadIdx.x >> 3)] = d;
     }
   }
-  staged();
-  // the wave's piece of dQ: d = 16*dg.., rows 16*rg..; its K^T operand
-  int dg = wave >> 1, rg = wave & 1, l4 = (lane & 15) >> 2, seg = lane & 3;
+  s16x8 vf[KG][4];
+  float bias[KG];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    int row = k * 32 + (lane >> 4) * 8 + l4;
-    int chunk = dg * 2 + (seg >> 1);
-    const char* x = ds01 + (seg & 1) * 8;
-    kt[k] = read_tr2(x + lds_at<64>(row, chunk),
-                     x + lds_at<64>(row + 4, chunk));
+  for (int n = 0; n < KG; ++n) {
+    int key = (wave + n * 4) * 32 + (lane & 31);
+    bias[n] = key < s.klen ? 0.f : -INFINITY;
+    keep<64>(a,
+             reinterpret_cast<const char*>(a.v.p) +
+                 2 * (s.batch * a.v.sb + s.kvh * a.v.sh + key * a.v.ss),
+             key < s.klen, lane, vf[n]);
   }
-  __syncthreads();  // K is read: the buffer is dS's
   float c = a.scale * kLog2e;
-  f32x16 dk[2] = {kNone, kNone}, dv[2] = {kNone, kNone};
+  f32x16 dk[KG][2], dv[KG][2];
+#pragma unroll
+  for (int n = 0; n < KG; ++n)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) dk[n][i] = dv[n][i] = kNone;
   int nk = (s.klen + 31) / 32;
+  staged();
 
-  auto step = [&](int t, char* dso) {
-    if (!live) return;
-    const char* qt = qall + Geo<64>::bytes(32) * t;
-    const char* dt = dall + Geo<64>::bytes(32) * t;
+  auto step = [&](int t, const char* qt, const char* dt) {
     const float *ls = lse + t * 32, *dl = del + t * 32;
-    f32x16 sc = kNone, dp = kNone;
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      sc = Op<T>::mfma(frag_row<64>(qt, 0, ks, lane), kf[ks], sc);
-      dp = Op<T>::mfma(frag_row<64>(dt, 0, ks, lane), vf[ks], dp);
-    }
-    if (cut)
+    for (int n = 0; n < KG; ++n) {
+      int grp = wave + n * 4;
+      if (grp >= nk) continue;
+      f32x16 sc = kNone, dp = kNone;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sc[i] = valid ? sc[i] : -INFINITY;
-    unsigned p[8], d[8];
+      for (int ks = 0; ks < 4; ++ks)
+        sc = Op<T>::mfma(frag_row<64>(qt, 0, ks, lane),
+                         frag_row<64>(kall, grp * 32, ks, lane), sc);
+      // keeps the operands of one product at a time in registers: spilled
+      // ones would have to wait for the tile's loads
+      
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float4 l4 = *reinterpret_cast<const float4*>(ls + j * 8 + h * 4);
-      float4 d4 = *reinterpret_cast<const float4*>(dl + j * 8 + h * 4);
-      const float *lp = &l4.x, *dd = &d4.x;
+      for (int ks = 0; ks < 4; ++ks)
+        dp = Op<T>::mfma(frag_row<64>(dt, 0, ks, lane), vf[n][ks], dp);
+      
+      // the products' operands leave the registers first
+      __builtin_amdgcn_sched_barrier(0);
+      unsigned p[8], d[8];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float x = __builtin_amdgcn_exp2f(
-            fmaf(sc[4 * j + 2 * i], c, -lp[2 * i]));
-        float y = __builtin_amdgcn_exp2f(
-            fmaf(sc[4 * j + 2 * i + 1], c, -lp[2 * i + 1]));
-        p[2 * j + i] = Op<T>::pack(x, y);
-        d[2 * j + i] =
-            Op<T>::pack(x * (dp[4 * j + 2 * i] - dd[2 * i]),
-                        y * (dp[4 * j + 2 * i + 1] - dd[2 * i + 1]));
+      for (int j = 0; j < 4; ++j) {
+        float4 l4 = *reinterpret_cast<const float4*>(ls + j * 8 + h * 4);
+        float4 d4 = *reinterpret_cast<const float4*>(dl + j * 8 + h * 4);
+        const float *lp = &l4.x, *dd = &d4.x;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          // a key that is not there has scores of 0 and a bias of -inf
+          float x = __builtin_amdgcn_exp2f(
+              fmaf(sc[4 * j + 2 * i], c, bias[n] - lp[2 * i]));
+          float y = __builtin_amdgcn_exp2f(
+              fmaf(sc[4 * j + 2 * i + 1], c, bias[n] - lp[2 * i + 1]));
+          p[2 * j + i] = Op<T>::pack(x, y);
+          d[2 * j + i] =
+              Op<T>::pack(x * (dp[4 * j + 2 * i] - dd[2 * i]),
+                          y * (dp[4 * j + 2 * i + 1] - dd[2 * i + 1]));
+        }
+        uint2 v = {d[2 * j], d[2 * j + 1]};
+        *reinterpret_cast<uint2*>(dso + grp * 32 * 64 +
+                                  ds_at(ln & 31, j * 8 + (ln >> 5) * 4)) = v;
       }
-      uint2 v = {d[2 * j], d[2 * j + 1]};
-      *reinterpret_cast<uint2*>(dso + key * 64 + ((j ^ perm2(key)) << 4) +
-                                ((h ^ ((key >> 3) & 1)) << 3)) = v;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          dv[n][i] = Op<T>::mfma(frag_col<64>(dt, k * 16, i, lane),
+                                 pack8(p + 4 * k), dv[n][i]);
+          dk[n][i] = Op<T>::mfma(frag_col<64>(qt, k * 16, i, lane),
+                                 pack8(d + 4 * k), dk[n][i]);
+        }
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        dv[i] = Op<T>::mfma(frag_col<64>(dt, k * 16, i, lane),
-                            pack8(p + 4 * k), dv[i]);
-        dk[i] = Op<T>::mfma(frag_col<64>(qt, k * 16, i, lane),
-                            pack8(d + 4 * k), dk[i]);
-      }
   };
-  auto put_dq = [&](int t, const char* dso) {
-    f32x4v acc = {0.f, 0.f, 0.f, 0.f};
-    int j = 2 * rg + (seg >> 1);
+  // columns 16 * wave.. of the tile's dQ
+  auto put_dq = [&](int t) {
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // its addresses are worked out anew
+    int l4 = (ln & 15) >> 2, seg = ln & 3;
+    f32x4v acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    int x = (ln >> 4) * 8 + l4;  // keys x.., x + 4.. of a group
+    const char* kc = kall + (seg & 1) * 8;
+    int chunk = wave * 2 + (seg >> 1);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < NKG; ++k) {
       if (k >= nk) break;
-      int x = k * 32 + (lane >> 4) * 8 + l4, y = x + 4;
-      acc = mfma16<T>(
-          kt[k],
-          read_tr2(dso + x * 64 + ((j ^ perm2(x)) << 4) +
-                       (((seg & 1) ^ ((x >> 3) & 1)) << 3),
-                   dso + y * 64 + ((j ^ perm2(y)) << 4) +
-                       (((seg & 1) ^ ((y >> 3) & 1)) << 3)),
-          acc);
+      s16x8 kt = read_tr2(kc + G::bytes(k * 32) + lds_at<64>(x, chunk),
+                          kc + G::bytes(k * 32) + lds_at<64>(x + 4, chunk));
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const char* d = dso + k * 32 * 64;
+        int r = u * 16 + seg * 4;
+        acc[u] = mfma16<T>(
+            kt, read_tr2(d + ds_at(x, r), d + ds_at(x + 4, r)), acc[u]);
+      }
     }
-    int r = t * 32 + rg * 16 + (lane & 15), e = dg * 16 + (lane >> 4) * 4;
-    int pos = (int)mdiv(r, a.g_mul, a.g_shift);
-    if (pos < a.sq && e < a.hd) {
-      uint2 v = {Op<T>::pack(acc[0] * a.scale, acc[1] * a.scale),
-                 Op<T>::pack(acc[2] * a.scale, acc[3] * a.scale)};
-      *reinterpret_cast<uint2*>(
-          reinterpret_cast<T*>(a.dq) +
-          (((long)s.batch * a.sq + pos) * a.hk * a.g + s.kvh * a.g + r -
-           pos * a.g) *
-              a.hd +
-          e) = v;
+    int e = wave * 16 + (ln >> 4) * 4;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      int r = t * 32 + u * 16 + (ln & 15);
+      int pos = (int)mdiv(r, a.g_mul, a.g_shift);
+      if (pos < a.sq && e < a.hd) {
+        uint2 v = {Op<T>::pack(acc[u][0] * a.scale, acc[u][1] * a.scale),
+                   Op<T>::pack(acc[u][2] * a.scale, acc[u][3] * a.scale)};
+        *reinterpret_cast<uint2*>(
+            reinterpret_cast<T*>(a.dq) +
+            (((long)s.batch * a.sq + pos) * a.hk * a.g + s.kvh * a.g + r -
+             pos * a.g) *
+                a.hd +
+            e) = v;
+      }
     }
+    __syncthreads();  // dS is read
   };
-  // one barrier a step: a step's dS is read after it, while the next step
-  // fills the other half
-  for (int t = 0; t < ntile; ++t) {
-    char* dso = ds01 + (t & 1) * 256 * 64;
-    step(t, dso);
-    __syncthreads();
-    put_dq(t, dso);
+  for (int t = 0; t < ntile; t += 2) {
+    if (t + 1 < ntile) load(t + 1, q1, d1);
+    step(t, q0, d0);
+    staged();
+    put_dq(t);
+    if (t + 1 >= ntile) break;
+    if (t + 2 < ntile) load(t + 2, q0, d0);
+    step(t + 1, q1, d1);
+    staged();
+    put_dq(t + 1);
   }
-  if (key >= a.sk) return;
-  long at = (((long)s.batch * a.sk + key) * a.hk + s.kvh) * a.hd;
-  put_row<T, 2>(reinterpret_cast<T*>(a.dv) + s.batch * a.vb + key * a.vs +
-                    s.kvh * a.vh,
-                dv, 1.f, a.hd, lane);
-  put_row<T, 2>(reinterpret_cast<T*>(a.dk) + at, dk, a.scale, a.hd, lane);
+#pragma unroll
+  for (int n = 0; n < KG; ++n) {
+    int key = (wave + n * 4) * 32 + (lane & 31);
+    if (key >= a.sk) continue;
+    if (key >= s.klen)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) dk[n][i] = dv[n][i] = kNone;
+    put_row<T, 2>(reinterpret_cast<T*>(a.dv) + s.batch * a.vb + key * a.vs +
+                      s.kvh * a.vh,
+                  dv[n], 1.f, a.hd, lane);
+    put_row<T, 2>(reinterpret_cast<T*>(a.dk) +
+                      (((long)s.batch * a.sk + key) * a.hk + s.kvh) * a.hd,
+                  dk[n], a.scale, a.hd, lane);
+  }
 }
 
 // x = scale * sums over the splits of part[split][nx + ny], then dv the sums
@@ -1189,6 +1266,7 @@ struct Plan {
   bool few;      // rows fit one wave: attn_rc_few_k, tiles of 32
   int dq, dkv;   // backward: parts over the keys, over the rows
   bool whole;    // backward in one pass: attn_rc_bwd_short_k
+  bool whole_fwd;  // all keys at once: attn_rc_fwd_short_k
   // free: no causal mask and no lengths
   Plan(long b, long sq, long sk, long hk, long g, long hd, bool free) {
     long bh = b * hk, rows = sq * g;
@@ -1197,6 +1275,10 @@ struct Plan {
     whole = free && hd <= 64 && sk > 64 && sk <= 256 && rows <= 256 &&
             bh >= 256;
     long rblk = bh * ((rows + 127) / 128), kblk = bh * ((sk + 127) / 128);
+    // two of its blocks a CU: 47 against 51 us at 1536 heads of 197 tokens,
+    // and no gain below
+    whole_fwd = hd <= 64 && sk <= 256 && rows > 128 &&
+                bh * ((rows + 255) / 256) >= 512;
     fwd = dq = dkv = 1;
     per = 0;
     few = false;
@@ -1229,7 +1311,7 @@ struct Plan {
 template <typename T, int HDT>
 void launch(const Args& a, int bwd, float* ws, hipStream_t s) {
   int rblk = (a.sq * a.g + 127) / 128, kblk = (a.sk + 127) / 128;
-  int bh = a.b * a.hk;
+  int bh = a.b * a.hk, rblk256 = (a.sq * a.g + 255) / 256;
   Plan p(a.b, a.sq, a.sk, a.hk, a.g, a.hd,
          !a.causal && !a.q_lens && !a.kv_lens);
   if (!bwd) {
@@ -1237,6 +1319,8 @@ void launch(const Args& a, int bwd, float* ws, hipStream_t s) {
     if (p.few)
       attn_rc_few_k<T, HDT>
           <<<bh * (p.fwd / 2), 128, 0, s>>>(a, p.fwd, p.per, ws);
+    else if (HDT == 64 && p.whole_fwd)
+      attn_rc_fwd_short_k<T><<<bh * rblk256, 512, 0, s>>>(a, rblk256);
     else
       attn_rc_fwd_k<T, HDT>
           <<<bh * rblk * p.fwd, 256, 0, s>>>(a, rblk, p.fwd, p.per, ws);
@@ -1248,7 +1332,12 @@ void launch(const Args& a, int bwd, float* ws, hipStream_t s) {
   }
   if constexpr (HDT == 64)
     if (p.whole) {
-      attn_rc_bwd_short_k<T><<<bh, 512, 0, s>>>(a);
+      if (a.sk <= 128)
+        attn_rc_bwd_short_k<T, 4><<<bh, 256, 0, s>>>(a);
+      else if (a.sk <= 224)
+        attn_rc_bwd_short_k<T, 7><<<bh, 256, 0, s>>>(a);
+      else
+        attn_rc_bwd_short_k<T, 8><<<bh, 256, 0, s>>>(a);
       return;
     }
   long nq = (long)a.b * a.sq * a.hk * a.g * a.hd;

@@ -137,7 +137,7 @@ std::vector<at::Tensor> qk_norm_rope(
               "q and k must be [b, s, heads, hd], alike but for the heads");
   long b = q.size(0), s = q.size(1), hd = q.size(3);
   TORCH_CHECK(hd >= 1 && hd <= 256, "head size must be 1 to 256, is ", hd);
-  TORCH_CHECK(b * s < (1l << 31) && q.size(2) + k.size(2) < 65536,
+  TORCH_CHECK(b * s < (1l << 31) - 65536 && q.size(2) + k.size(2) < 65536,
               "too many rows");
   bool bwd = dq.has_value();
   TORCH_CHECK(bwd == dk.has_value(), "dq and dk come together");

@@ -36,10 +36,34 @@ struct Args {
   const void* pos;         // [b, s] int64 / int32, null: the row's index
   int pos32;
   int npos, rot, hd, s;
-  long tokens;
+  int tokens;  // b * s, below 2^31 less the grid's stride
   float eps;
   int slices;  // waves that share a token's heads (forward)
 };
+
+// Where the 8 elements of token (b, srow), head j (queries, then keys), chunk
+// lie: the token is the wave's, so its parts are scalars and a lane only
+// chooses between the two tensors.
+enum Which { X, DY, Y };
+template <typename T, Which W>
+DEV_INLINE T* at_head(const Args& a, long b, int srow, int j, int chunk) {
+  auto base = [&](const HeadsIn& t) {
+    if (W == X)
+      return const_cast<T*>(reinterpret_cast<const T*>(t.x)) + b * t.sb +
+             srow * t.ss;
+    if (W == DY)
+      return const_cast<T*>(reinterpret_cast<const T*>(t.dy)) + b * t.gb +
+             srow * t.gs;
+    return reinterpret_cast<T*>(t.y) + b * t.yb + srow * t.ys;
+  };
+  auto stride = [](const HeadsIn& t) {
+    return W == X ? t.sh : W == DY ? t.gh : t.yh;
+  };
+  T *q = base(a.t[0]), *k = base(a.t[1]) - a.t[0].heads * stride(a.t[1]);
+  long sq = stride(a.t[0]), sk = stride(a.t[1]);
+  bool isk = j >= a.t[0].heads;
+  return (isk ? k : q) + j * (isk ? sk : sq) + chunk * 8;
+}
 
 // a position outside the tables turns by NaN: the result shows it
 DEV_INLINE int position(const Args& a, long tok, int srow) {
@@ -117,14 +141,15 @@ struct Turn {
 template <typename T, int G, bool INTER>
 __global__ __launch_bounds__(256) void qknorm_fwd_k(Args a) {
   int lane = threadIdx.x & 63;
-  long wv = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  long tok = wv / a.slices;
+  unsigned wv = blockIdx.x * 4 +
+                __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int tok = wv / (unsigned)a.slices;
   if (tok >= a.tokens) return;
-  int slice = (int)(wv - tok * a.slices);
+  int slice = wv - tok * a.slices;
   int chunk = lane & (G - 1), grp = lane / G;
   bool act = chunk * 8 < a.hd;
-  long b = tok / a.s;
-  int srow = (int)(tok - b * a.s);
+  int b = __builtin_amdgcn_readfirstlane(tok / a.s);
+  int srow = tok - b * a.s;
   Turn<INTER> turn;
   if (a.rot) turn.load(a, position(a, tok, srow), chunk, lane);
   float w[2][8];
@@ -147,14 +172,11 @@ __global__ __launch_bounds__(256) void qknorm_fwd_k(Args a) {
     int j = j0 + grp;
     bool isk = j >= a.t[0].heads;
     bool live = act && j < nv;
-    const HeadsIn& t = a.t[isk ? 1 : 0];
-    int head = isk ? j - a.t[0].heads : j;
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = 0.f;
     if (live) {
-      Vec8<T> v = load8(reinterpret_cast<const T*>(t.x) + b * t.sb +
-                        srow * t.ss + head * t.sh + chunk * 8);
+      Vec8<T> v = load8(at_head<T, X>(a, b, srow, j, chunk));
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = to_f32(v.v[i]);
     }
@@ -171,9 +193,7 @@ __global__ __launch_bounds__(256) void qknorm_fwd_k(Args a) {
       Vec8<T> v;
 #pragma unroll
       for (int i = 0; i < 8; ++i) v.v[i] = from_f32<T>(x[i]);
-      store8(reinterpret_cast<T*>(t.y) + b * t.yb + srow * t.ys +
-                 head * t.yh + chunk * 8,
-             v);
+      store8(at_head<T, Y>(a, b, srow, j, chunk), v);
     }
   }
 }
@@ -183,7 +203,8 @@ template <typename T, int G, bool INTER>
 __global__ __launch_bounds__(256) void qknorm_bwd_k(Args a,
                                                     float* __restrict__ part) {
   __shared__ float red[4][2][G * 8];
-  int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int lane = threadIdx.x & 63;
+  int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int chunk = lane & (G - 1), grp = lane / G;
   bool act = chunk * 8 < a.hd;
   bool norm = a.t[0].w != nullptr;
@@ -201,32 +222,56 @@ __global__ __launch_bounds__(256) void qknorm_bwd_k(Args a,
     }
   float inv_hd = 1.f / (float)a.hd;
   int nv = a.t[0].heads + a.t[1].heads;
-  for (long tok = (long)blockIdx.x * 4 + wave; tok < a.tokens;
-       tok += (long)gridDim.x * 4) {
-    long b = tok / a.s;
-    int srow = (int)(tok - b * a.s);
+  // One step ahead: the loads of the next heads (and of the next token's
+  // angles) are out while these are worked on; without that, 16 waves a CU
+  // keep too few bytes in flight.
+  struct Raw {
+    Vec8<T> x, d;
+  };
+  struct Token {
+    int at, b, row;
+  };
+  auto token = [&](int at) {
+    int b = __builtin_amdgcn_readfirstlane(at / a.s);
+    return Token{at, b, at - b * a.s};
+  };
+  if ((int)blockIdx.x * 4 + wave < a.tokens) {
+    auto fetch = [&](const Token& t, int j0, Raw& r) {
+      int j = j0 + grp;
+      if (!act || j >= nv) return;
+      r.d = load8(at_head<T, DY>(a, t.b, t.row, j, chunk));
+      if (norm) r.x = load8(at_head<T, X>(a, t.b, t.row, j, chunk));
+    };
+    auto angles = [&](const Token& t, Turn<INTER>& turn) {
+      if (a.rot) turn.load(a, position(a, t.at, t.row), chunk, lane);
+    };
+    Raw raw;
     Turn<INTER> turn;
-    if (a.rot) turn.load(a, position(a, tok, srow), chunk, lane);
-    for (int j0 = 0; j0 < nv; j0 += 64 / G) {
+    Token tok = token(blockIdx.x * 4 + wave);
+    angles(tok, turn);
+    fetch(tok, 0, raw);
+    for (int j0 = 0;;) {
+      int nj = j0 + 64 / G;
+      Token nt = tok;
+      if (nj >= nv) {
+        nj = 0;
+        nt = token(tok.at + gridDim.x * 4);
+      }
+      bool more = nt.at < a.tokens;
+      Raw next;
+      Turn<INTER> nturn;
+      if (more) {
+        fetch(nt, nj, next);
+        if (nj == 0) angles(nt, nturn);
+      }
       int j = j0 + grp;
       bool isk = j >= a.t[0].heads;
       bool live = act && j < nv;
-      const HeadsIn& t = a.t[isk ? 1 : 0];
-      int head = isk ? j - a.t[0].heads : j;
       float x[8], g[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = g[i] = 0.f;
-      if (live) {
-        Vec8<T> d = load8(reinterpret_cast<const T*>(t.dy) + b * t.gb +
-                          srow * t.gs + head * t.gh + chunk * 8);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = to_f32(d.v[i]);
-        if (norm) {
-          Vec8<T> v = load8(reinterpret_cast<const T*>(t.x) + b * t.sb +
-                            srow * t.ss + head * t.sh + chunk * 8);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = to_f32(v.v[i]);
-        }
+      for (int i = 0; i < 8; ++i) {
+        x[i] = live && norm ? to_f32(raw.x.v[i]) : 0.f;
+        g[i] = live ? to_f32(raw.d.v[i]) : 0.f;
       }
       if (a.rot) turn.template apply<true>(g);
       if (norm) {
@@ -252,10 +297,13 @@ __global__ __launch_bounds__(256) void qknorm_bwd_k(Args a,
         Vec8<T> v;
 #pragma unroll
         for (int i = 0; i < 8; ++i) v.v[i] = from_f32<T>(g[i]);
-        store8(reinterpret_cast<T*>(t.y) + b * t.yb + srow * t.ys +
-                   head * t.yh + chunk * 8,
-               v);
+        store8(at_head<T, Y>(a, tok.b, tok.row, j, chunk), v);
       }
+      if (!more) break;
+      raw = next;
+      if (nj == 0) turn = nturn;
+      tok = nt;
+      j0 = nj;
     }
   }
   if (!norm) return;
@@ -292,7 +340,7 @@ __global__ __launch_bounds__(256) void qknorm_any_k(Args a, int inter,
 #pragma unroll
   for (int k = 0; k < 4; ++k) acc[0][k] = acc[1][k] = 0.f;
   float inv_hd = 1.f / (float)a.hd;
-  long total = a.tokens * nv;
+  long total = (long)a.tokens * nv;
   for (long u = (long)blockIdx.x * 4 + wave; u < total;
        u += (long)gridDim.x * 4) {
     long tok = u / nv;
@@ -451,7 +499,7 @@ void pdta_qknorm(const void* const* x, const long* xs, const void* const* dy,
               w[k], y[k], ys[3 * k], ys[3 * k + 1], ys[3 * k + 2],
               heads[k]};
   a.cos = cos, a.sin = sin, a.pos = pos, a.pos32 = pos32, a.npos = npos;
-  a.rot = rot, a.hd = hd, a.s = (int)s_len, a.tokens = b * s_len;
+  a.rot = rot, a.hd = hd, a.s = (int)s_len, a.tokens = (int)(b * s_len);
   a.eps = eps, a.slices = 1;
   int nv = heads[0] + heads[1];
   if (a.tokens == 0 || nv == 0) return;
@@ -465,7 +513,7 @@ void pdta_qknorm(const void* const* x, const long* xs, const void* const* dy,
       int most = (nv + 64 / G - 1) / (64 / G);
       long want = (2048 + a.tokens - 1) / a.tokens;
       a.slices = (int)(want < most ? want : most);
-      blocks = (int)((a.tokens * a.slices + 3) / 4);
+      blocks = (int)(((long)a.tokens * a.slices + 3) / 4);
     }
     PDTA_DISPATCH_DTYPE(dt, T, {
       if (G == 4)

@@ -646,33 +646,54 @@ __global__ __launch_bounds__(128, 2) void attn_rc_few_k(Args a, int parts,
   run.put(a, s, row, bh, parts, at, part, lane);
 }
 
-// out = sum over parts of exp2(lse_p - lse) out_p, lse = log2 sum exp2(lse_p);
-// 32 lanes a row. A part that saw no key has lse +inf and no output.
+// out = sum over parts of exp2(lse_p - lse) out_p, lse = log2 sum exp2(lse_p).
+// A block a row: 8 groups of 32 lanes take the parts in turn, so that all of
+// a row's loads are out at once. Parts that saw no key have lse +inf and no
+// output; they come last, as parts take the keys in order.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_rc_join_rows_k(Args a, int parts,
                                                            const float* part) {
+  __shared__ float4 accs[8][32];
+  __shared__ float sums[8];
   long rows = (long)a.b * a.hk * a.sq * a.g;
-  long r = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (r >= rows) return;
-  int d = (threadIdx.x & 31) * 4;
+  long r = blockIdx.x;
+  int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, d = lane * 4;
   const float* ls = part + parts * rows * a.hd + r;
   float top = -INFINITY;
-  for (int p = 0; p < parts; ++p) {
+  int used = 0;
+  for (int p = lane; p < parts; p += 32) {
     float l = ls[p * rows];
-    if (l != INFINITY) top = fmaxf(top, l);
+    if (l != INFINITY) {
+      top = fmaxf(top, l);
+      used = p + 1;
+    }
+  }
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    top = fmaxf(top, __shfl_xor(top, m, 64));
+    int o = __shfl_xor(used, m, 64);
+    used = o > used ? o : used;
   }
   float sum = 0.f;
   float4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < parts; ++p) {
-    float l = ls[p * rows];
-    if (l == INFINITY) continue;
-    float w = __builtin_amdgcn_exp2f(l - top);
+  int at = d < a.hd ? d : 0;  // lanes past the head load and drop its start
+#pragma unroll 4
+  for (int p = grp; p < used; p += 8) {
+    float w = __builtin_amdgcn_exp2f(ls[p * rows] - top);
+    float4 x =
+        *reinterpret_cast<const float4*>(part + (p * rows + r) * a.hd + at);
     sum += w;
-    if (d < a.hd) {
-      float4 x = *reinterpret_cast<const float4*>(part +
-                                                  (p * rows + r) * a.hd + d);
-      acc.x += w * x.x, acc.y += w * x.y, acc.z += w * x.z, acc.w += w * x.w;
-    }
+    acc.x += w * x.x, acc.y += w * x.y, acc.z += w * x.z, acc.w += w * x.w;
+  }
+  accs[grp][lane] = acc;
+  if (lane == 0) sums[grp] = sum;
+  __syncthreads();
+  if (grp) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) {
+    float4 x = accs[k][lane];
+    sum += sums[k];
+    acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
   }
   float m = sum != 0.f ? 1.f / sum : 0.f;
   int n = a.sq * a.g;
@@ -686,7 +707,7 @@ __global__ __launch_bounds__(256) void attn_rc_join_rows_k(Args a, int parts,
         reinterpret_cast<T*>(a.out) +
         (((long)batch * a.sq + pos) * a.hk * a.g + head) * a.hd + d) = v;
   }
-  if (d == 0 && a.lse)
+  if (lane == 0 && a.lse)
     a.lse[r] = sum != 0.f ? top + __builtin_amdgcn_logf(sum) : INFINITY;
 }
 
@@ -1326,7 +1347,7 @@ void launch(const Args& a, int bwd, float* ws, hipStream_t s) {
           <<<bh * rblk * p.fwd, 256, 0, s>>>(a, rblk, p.fwd, p.per, ws);
     if (p.fwd > 1) {
       long rows = (long)bh * a.sq * a.g;
-      attn_rc_join_rows_k<T><<<(rows + 7) / 8, 256, 0, s>>>(a, p.fwd, ws);
+      attn_rc_join_rows_k<T><<<rows, 256, 0, s>>>(a, p.fwd, ws);
     }
     return;
   }

@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from .backend import ext
 
@@ -935,6 +936,7 @@ class AttentionRecomputeFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, q_lens, kv_lens = ctx.saved_tensors
         scale, causal = ctx.scale, ctx.causal
@@ -980,11 +982,12 @@ def attention_recompute(q, k, v, scale: float | None = None,
     scale: positive, None for 1/sqrt(hd).
     q_lens, kv_lens: int32 or int64 [b], the sequences' lengths (None: sq,
     sk); cut to 0..sq, 0..sk. What lies behind them is never read; outputs
-    and gradients there are 0.
+    and gradients there are 0. Inside them v has to be finite: a probability
+    of 0 does not keep a NaN or an infinity in it from earlier queries.
     causal: query i sees keys up to i + kv_len - q_len, so the last query
     sees the last key. A query that sees none gives 0.
     GPU (csrc/attn_recompute.hip): bf16 and fp16, hd a multiple of 8 up to
-    128; one launch forward, two backward; results do not depend on timing.
+    128; results do not depend on timing; no gradient of the gradient.
     In fp16, gradients need a loss scale that keeps dS in its range, as the
     fp16 training path has."""
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape \
@@ -1111,6 +1114,7 @@ class QKNormRopeFn(torch.autograd.Function):
         return one(q, wq), one(k, wk)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
 
@@ -1212,6 +1216,7 @@ class AttentionQKVRopeFn(torch.autograd.Function):
         return out.view(b, s, h * hd)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         qkv2d, wq, wk, cos, sin, qn, kn, out, lse = ctx.saved_tensors
         b, s, h, hd, scale, causal, eps = ctx.dims

@@ -365,3 +365,34 @@ def test_refuses_what_the_kernel_cannot_take():
     q = torch.zeros(1, 4, 2, 64, device="cuda", dtype=torch.bfloat16)
     with pytest.raises(ValueError):
         OF.attention_recompute(q, q, q, kv_lens=torch.tensor([4]))
+
+
+@pytest.mark.parametrize("dev,dtype", [
+    ("cpu", torch.float32),
+    pytest.param("cuda", torch.bfloat16, marks=gpu)])
+def test_no_gradient_of_the_gradient(dev, dtype):
+    q = torch.randn(1, 70, 2, 64, device=dev, dtype=dtype,
+                    requires_grad=True)
+    with pytest.raises(RuntimeError):
+        out = OF.attention_recompute(q, q, q).float().square().sum()
+        g, = torch.autograd.grad(out, q, create_graph=True)
+        g.float().sum().backward()
+    w = torch.ones(64, device=dev, requires_grad=True)
+    with pytest.raises(RuntimeError):
+        out = OF.qk_norm_rope(q, q, w, w)[0].float().square().sum()
+        g, = torch.autograd.grad(out, q, create_graph=True)
+        g.float().sum().backward()
+
+
+@gpu
+def test_one_gradient_of_several():
+    """Only k's gradient is asked for, as a frozen projection would."""
+    q, k, v, do = _inputs("cuda", torch.bfloat16, 2, 90, 90, 4, 2, 64)
+    want = _run(q, k, v, do, causal=True)
+    leaf = k.clone().requires_grad_(True)
+    out = OF.attention_recompute(q, leaf, v, causal=True)
+    g, = torch.autograd.grad(out, leaf, do)
+    assert torch.equal(g, want[2]) and torch.equal(out, want[0])
+    with torch.inference_mode():
+        assert torch.equal(OF.attention_recompute(q, k, v, causal=True),
+                           want[0])

@@ -121,7 +121,9 @@ struct Seq {
 };
 
 // Block index -> sequence and head, block of it, and part. Causal: all heads'
-// longest blocks first (LAST: high indexes are long). Else 8 heads at a time.
+// longest blocks first (LAST: high indexes are long). Else 8 heads at a time
+// (also with lengths: the longest blocks of all sequences first put long
+// blocks together on a CU and took 20% more).
 // Either way a head's blocks are 8 (or bh) apart, and as the hardware deals
 // blocks out to its 8 dies in turn, they meet in one die's L2.
 DEV_INLINE void place(const Args& a, int nblk, bool last, int* bh, int* blk) {
@@ -647,17 +649,20 @@ __global__ __launch_bounds__(128, 2) void attn_rc_few_k(Args a, int parts,
 }
 
 // out = sum over parts of exp2(lse_p - lse) out_p, lse = log2 sum exp2(lse_p).
-// A block a row: 8 groups of 32 lanes take the parts in turn, so that all of
-// a row's loads are out at once. Parts that saw no key have lse +inf and no
-// output; they come last, as parts take the keys in order.
-template <typename T>
+// Groups of 32 lanes, GPR of the block's 8 a row: with many parts a row has
+// all 8, which take the parts in turn, so that all of its loads are out at
+// once; with 8 parts or fewer each group has a row. Parts that saw no key have
+// lse +inf and no output; they come last, as parts take the keys in order.
+template <typename T, int GPR>
 __global__ __launch_bounds__(256) void attn_rc_join_rows_k(Args a, int parts,
                                                            const float* part) {
   __shared__ float4 accs[8][32];
   __shared__ float sums[8];
   long rows = (long)a.b * a.hk * a.sq * a.g;
-  long r = blockIdx.x;
   int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, d = lane * 4;
+  long r = (long)blockIdx.x * (8 / GPR) + grp / GPR;
+  grp %= GPR;
+  if (GPR < 8 && r >= rows) return;
   const float* ls = part + parts * rows * a.hd + r;
   float top = -INFINITY;
   int used = 0;
@@ -678,22 +683,24 @@ __global__ __launch_bounds__(256) void attn_rc_join_rows_k(Args a, int parts,
   float4 acc = {0.f, 0.f, 0.f, 0.f};
   int at = d < a.hd ? d : 0;  // lanes past the head load and drop its start
 #pragma unroll 4
-  for (int p = grp; p < used; p += 8) {
+  for (int p = grp; p < used; p += GPR) {
     float w = __builtin_amdgcn_exp2f(ls[p * rows] - top);
     float4 x =
         *reinterpret_cast<const float4*>(part + (p * rows + r) * a.hd + at);
     sum += w;
     acc.x += w * x.x, acc.y += w * x.y, acc.z += w * x.z, acc.w += w * x.w;
   }
-  accs[grp][lane] = acc;
-  if (lane == 0) sums[grp] = sum;
-  __syncthreads();
-  if (grp) return;
+  if (GPR == 8) {
+    accs[grp][lane] = acc;
+    if (lane == 0) sums[grp] = sum;
+    __syncthreads();
+    if (grp) return;
 #pragma unroll
-  for (int k = 1; k < 8; ++k) {
-    float4 x = accs[k][lane];
-    sum += sums[k];
-    acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+    for (int k = 1; k < 8; ++k) {
+      float4 x = accs[k][lane];
+      sum += sums[k];
+      acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+    }
   }
   float m = sum != 0.f ? 1.f / sum : 0.f;
   int n = a.sq * a.g;
@@ -1315,16 +1322,16 @@ struct Plan {
       fwd = (int)((tiles + 2 * run - 1) / (2 * run)) * 2;
     } else {
       long tiles = (sk + TILE - 1) / TILE;
-      fwd = clamp(1024 / rblk, tiles / 8);
+      fwd = rblk < 512 ? clamp(1024 / rblk, tiles / 8, 64) : 1;
       per = (int)((tiles + fwd - 1) / fwd);
     }
-    dq = clamp(1024 / rblk, sk / 512);
+    dq = rblk < 512 ? clamp(1024 / rblk, sk / 512, 64) : 1;
     // a causal mask's blocks differ in length: more rounds even them out
-    dkv = clamp((1024 + kblk - 1) / kblk, rows / 512);
+    dkv = clamp((1024 + kblk - 1) / kblk, rows / 512, 16);
   }
-  static int clamp(long want, long most) {
+  static int clamp(long want, long most, long cap) {
     long n = want < most ? want : most;
-    n = n < 16 ? n : 16;
+    n = n < cap ? n : cap;
     return n < 1 ? 1 : (int)n;
   }
 };
@@ -1347,7 +1354,11 @@ void launch(const Args& a, int bwd, float* ws, hipStream_t s) {
           <<<bh * rblk * p.fwd, 256, 0, s>>>(a, rblk, p.fwd, p.per, ws);
     if (p.fwd > 1) {
       long rows = (long)bh * a.sq * a.g;
-      attn_rc_join_rows_k<T><<<rows, 256, 0, s>>>(a, p.fwd, ws);
+      if (p.fwd > 8)
+        attn_rc_join_rows_k<T, 8><<<rows, 256, 0, s>>>(a, p.fwd, ws);
+      else
+        attn_rc_join_rows_k<T, 1>
+            <<<(rows + 7) / 8, 256, 0, s>>>(a, p.fwd, ws);
     }
     return;
   }

@@ -297,7 +297,7 @@ AttnShape attn_check(const at::Tensor& q, const at::Tensor& k,
   }
   long g = n.hk ? n.h / n.hk : 1;
   TORCH_CHECK((n.sq + n.sk + 1024) * g < (1l << 31) &&
-                  n.b * n.hk * ((n.sq * g + n.sk) / 128 + 2) * 16 <
+                  n.b * n.hk * ((n.sq * g + n.sk) / 128 + 2) * 64 <
                       (1l << 31),
               "attention: too many rows");
   for (const auto* l : {&q_lens, &kv_lens})

@@ -870,7 +870,7 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk,
 // With few key blocks the rows are dealt out to `nsplit` blocks in turn
 // (tile t to block t % nsplit), whose fp32 sums a last kernel adds.
 template <typename T, int HDT>
-__global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
+__global__ __launch_bounds__(256, HDT == 64 ? 3 : 2) void attn_rc_dkv_k(Args a, int nblk,
                                                         int nsplit,
                                                         float* part) {
   using G = Geo<HDT>;
@@ -942,6 +942,8 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
   auto step = [&](int t, const char* qt, const char* dt, const char* sd) {
     const float* ls = reinterpret_cast<const float*>(sd);
     const float* ds = ls + 64;
+    int ln = lane;  // some addresses are worked out anew, for registers
+    asm volatile("" : "+v"(ln));
 #pragma unroll
     for (int u = 0; u < RT / 32; ++u) {
       int r0 = first + t * RT + u * 32;
@@ -985,9 +987,9 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dkv_k(Args a, int nblk,
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int i = 0; i < G::DT; ++i) {
-          dv[i] = Op<T>::mfma(frag_col<HDT>(dt, u * 32 + k * 16, i, lane),
+          dv[i] = Op<T>::mfma(frag_col<HDT>(dt, u * 32 + k * 16, i, ln),
                               pack8(p + 4 * k), dv[i]);
-          dk[i] = Op<T>::mfma(frag_col<HDT>(qt, u * 32 + k * 16, i, lane),
+          dk[i] = Op<T>::mfma(frag_col<HDT>(qt, u * 32 + k * 16, i, ln),
                               pack8(d + 4 * k), dk[i]);
         }
     }

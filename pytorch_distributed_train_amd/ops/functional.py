@@ -1187,8 +1187,9 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None,
             positions.shape != (b, s)
             or positions.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"positions must be int32 or int64 [{b}, {s}]")
-    if positions is not None:
-        positions = positions.contiguous()
+    positions, cos, sin, q_weight, k_weight = (
+        x if x is None else x.contiguous()
+        for x in (positions, cos, sin, q_weight, k_weight))
     if q.is_cuda:
         return tuple(ext().qk_norm_rope_grad(q, k, q_weight, k_weight, cos,
                                              sin, positions, eps,
@@ -1332,7 +1333,7 @@ def adamw_step(p, g, m, v, step, lr, beta1=0.9, beta2=0.999, eps=1e-8,
 
     step: one int64 on p's device, advanced here, so a captured step replays
     as the next one. lr: a number, or one float32 on p's device.
-    decay: None, or uint8 [n/64], 0 where weight decay is left out.
+    decay: None, or uint8 [n/64], 1 where weight decay applies, 0 elsewhere.
     States: m, v fp32; or, with m_scale and v_scale (fp32 [n/64]),
     float8_e4m3fn of m and of sqrt(v) over a scale per 64 elements, sqrt(v)
     rounded up or down at random by a mix of element, step and seed. A

@@ -238,14 +238,25 @@ class FusedAdamW:
     @torch.no_grad()
     def load_state_dict(self, sd: dict) -> None:
         g = sd["param_groups"][0]
+        if "betas" not in g:
+            raise ValueError("not the state of an AdamW optimizer")
         if g.get("amsgrad") or g.get("maximize"):
             raise ValueError("amsgrad and maximize are not supported")
+        if any(not 0 <= int(i) < self.flat.num_params for i in sd["state"]):
+            raise ValueError(f"state of {len(sd['state'])} parameters for "
+                             f"{self.flat.num_params}")
         self.lr = g["lr"]
         self.betas = tuple(float(b) for b in g["betas"])
         self.eps = g["eps"]
         self.weight_decay = g["weight_decay"]
         self.seed = int(g.get("seed", self.seed))
         dev = self.flat.master.device
+        # parameters that the state does not hold have none
+        self.step_count.zero_()
+        for t in (self.exp_avg, self.exp_avg_sq, self.exp_avg_scale,
+                  self.exp_avg_sq_scale):
+            if t is not None:
+                t.view(torch.uint8).zero_()
         for i, s in sd["state"].items():
             i = int(i)
             off, n = self.flat.offsets[i], self.flat.sizes[i]

@@ -301,11 +301,48 @@ def test_refusals(dev):
         FusedAdamW(flat, lr=0.1, betas=(0.9, 1.0))
 
 
-def test_empty():
-    z = torch.zeros(0)
-    step = torch.zeros(1, dtype=torch.int64)
+@pytest.mark.parametrize("dev", DEVICES)
+def test_empty(dev):
+    z = torch.zeros(0, device=dev)
+    step = torch.zeros(1, dtype=torch.int64, device=dev)
     OF.adamw_step(z, z, z, z, step, 0.1)
     assert int(step) == 1
+
+
+def test_load_state_dict_replaces_and_refuses():
+    from pytorch_distributed_train_amd.parallel.optim import FusedSGD
+    flat = FlatParams(_model().named_parameters())
+    for bits in (8, 32):
+        opt = FusedAdamW(flat, lr=0.1, state_bits=bits)
+        _flat_grads(flat, 1)
+        opt.step()
+        sd = opt.state_dict()
+        opt.step()
+        only = {**sd, "state": {0: sd["state"][0]}}
+        opt.load_state_dict(only)
+        assert int(opt.step_count) == 1
+        off = flat.offsets[1]
+        assert not bool(opt.exp_avg[off:].float().any())
+        assert bool(opt.exp_avg[:off].float().any())
+        opt.load_state_dict({**sd, "state": {}})
+        assert int(opt.step_count) == 0
+        assert not bool(opt.exp_avg_sq.float().any())
+        with pytest.raises(ValueError):
+            opt.load_state_dict({**sd, "state": {99: sd["state"][0]}})
+        with pytest.raises(ValueError):
+            opt.load_state_dict(FusedSGD(flat, 0.1, 0.9).state_dict())
+
+
+def test_ranks_stay_alike_with_8bit_states(tmp_path):
+    """The random rounding is the same on every rank."""
+    from test_ddp_gloo import _run_workers
+    _run_workers(False, False, tmp_path,
+                 ("--optimizer", "adamw", "--adam-bits", "8", "--lr",
+                  "0.001"))
+    a, b = (torch.load(str(tmp_path / f"rank{r}.pt"), weights_only=True)
+            for r in range(2))
+    assert torch.equal(a["grad"], b["grad"])
+    assert torch.equal(a["master"], b["master"])
 
 
 @gpu

@@ -138,6 +138,13 @@ CASES = [
     (1, 700, 1100, 2, 1, 64, True, None, None),
     (1, 1025, 1025, 4, 2, 128, True, None, None),
     (3, 5, 2000, 2, 1, 128, True, None, [2000, 3, 777]),
+    (2, 90, 70, 2, 2, 120, False, [90, 31], None),   # lengths of one side
+    (2, 70, 200, 3, 1, 56, True, [1, 66], None),
+    # 12 and 7 heads a key head: rows of a load that straddle positions
+    (1, 37, 150, 12, 1, 64, True, None, None),
+    (1, 37, 150, 12, 1, 128, False, None, None),
+    (2, 21, 99, 14, 2, 88, True, None, [99, 40]),
+    (1, 40, 60, 32, 1, 64, False, None, None),
     # many heads of 65 to 256 keys: backward in one pass
     (64, 197, 197, 4, 4, 64, False, None, None),
     (128, 70, 130, 6, 2, 40, False, None, None),
@@ -283,6 +290,50 @@ def test_offsets_past_32_bits():
         views.append(at)
     for u, w in zip(_run(*views), _run(q, k, v, do)):
         assert torch.equal(u, w)
+
+
+@gpu
+def test_rows_far_apart():
+    """Rows a quarter of 2^32 bytes apart: past a load's 32-bit offsets."""
+    step = (1 << 28) + 64
+    big = torch.empty(3 * step, dtype=torch.bfloat16, device="cuda")
+    q, k, v, do = _inputs("cuda", torch.bfloat16, 1, 3, 3, 1, 1, 64)
+    views = []
+    for i, x in enumerate((q, k, v, do)):
+        at = big.as_strided(x.shape, (3 * step, step, 64, 1), i * 64)
+        at.copy_(x)
+        views.append(at)
+    for u, w in zip(_run(*views), _run(q, k, v, do)):
+        assert torch.equal(u, w)
+
+
+@gpu
+@pytest.mark.parametrize("b,s,h,causal", [(1, 1030, 2, True),
+                                          (64, 130, 4, False),
+                                          (2, 70, 3, True)])
+def test_over_one_projection(b, s, h, causal):
+    """attention_qkv_rope does what the two operators do, in the parts of
+    one projection's gradient (with the rows dealt out, in one pass, and
+    plainly)."""
+    hd = 64
+    g = torch.Generator().manual_seed(s)
+    qkv = torch.randn(b * s, 3 * h * hd, generator=g).to(torch.bfloat16) \
+        .cuda()
+    w = [(1 + 0.2 * torch.randn(hd, generator=g)).cuda() for _ in range(2)]
+    do = torch.randn(b, s, h * hd, generator=g).to(torch.bfloat16).cuda()
+    cos, sin = OF.rope_tables(s, hd, device="cuda")
+    leaves = [x.requires_grad_(True) for x in (qkv, *w)]
+    out = OF.attention_qkv_rope(*leaves, cos, sin, b, s, h, hd,
+                                causal=causal)
+    got = [out, *torch.autograd.grad(out, leaves, do)]
+    q, k, v = leaves[0].view(b, s, 3, h, hd).unbind(2)
+    q, k = OF.qk_norm_rope(q, k, leaves[1], leaves[2], cos, sin)
+    out = OF.attention_recompute(q, k, v, causal=causal).view(b, s, h * hd)
+    want = [out, *torch.autograd.grad(out, leaves, do)]
+    for a, c in zip(got, want):
+        assert torch.equal(a, c)
+    with pytest.raises(ValueError):
+        OF.attention_qkv_rope(*leaves, cos, sin, b, s + 1, h, hd)
 
 
 @gpu

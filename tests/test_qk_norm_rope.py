@@ -279,3 +279,31 @@ def test_captured_and_on_another_stream():
         torch.cuda.synchronize()
         for a, b in zip(out, want):
             assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_one_of_two_results_used(dev):
+    """No gradient for k' and none asked for the weights."""
+    q, k, wq, wk, cos, sin, _, dq, _ = _case(
+        dev, torch.float32, 2, 9, 3, 1, 64, 64, False, None, True)
+    a, b = (x.detach().requires_grad_(True) for x in (q, k))
+    y, _ = OF.qk_norm_rope(a, b, wq, wk, cos, sin)
+    ga, gb = torch.autograd.grad(y, (a, b), dq, allow_unused=True)
+    y2, _ = OF.qk_norm_rope(a, k, wq, wk, cos, sin)
+    assert torch.equal(ga, torch.autograd.grad(y2, a, dq)[0])
+    assert gb is None or not bool(gb.any())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_tables_and_weights_of_any_stride(dev):
+    q, k, wq, wk, cos, sin, p, _, _ = _case(
+        dev, torch.float32, 2, 9, 3, 1, 64, 64, False, torch.int64, True)
+    want = OF.qk_norm_rope(q, k, wq, wk, cos, sin, positions=p)
+
+    def odd(x):  # the same values, every second element of a wider tensor
+        return torch.stack([x, torch.zeros_like(x)], -1)[..., 0]
+
+    got = OF.qk_norm_rope(q, k, odd(wq), odd(wk), odd(cos), odd(sin),
+                          positions=odd(p))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

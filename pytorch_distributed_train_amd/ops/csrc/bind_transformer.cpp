@@ -5,6 +5,7 @@
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <hip/hip_runtime_api.h>
 
@@ -440,6 +441,28 @@ void once(const char* what) {
               ": a gradient of the gradient is not supported");
 }
 
+// A leaf keeps one node that gathers its gradient, with the stream that was
+// current when the node was made, for as long as any graph holds it. If that
+// is the default stream and a backward pass is captured on another, autograd
+// makes the default stream wait for the capture, which ends the process. A
+// forward that would lead there is refused.
+void capture_check(const std::vector<at::Tensor>& leaves) {
+  if (!at::GradMode::is_enabled()) return;
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(cur_stream(), &st) != hipSuccess ||
+      st == hipStreamCaptureStatusNone)
+    return;
+  for (const at::Tensor& t : leaves) {
+    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+    auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) continue;
+    auto s = node->stream();
+    TORCH_CHECK(!s.has_value() || s->id() != 0,
+                "captured with a gradient: another graph of the same leaf, "
+                "made on the default stream, is alive; delete it first");
+  }
+}
+
 // t itself if 16-byte accesses can walk its rows
 at::Tensor walkable(const at::Tensor& t) {
   return t.dim() == 4 && t.stride(3) == 1 && rows8(t) ? t : t.contiguous();
@@ -477,6 +500,8 @@ at::Tensor attention_recompute(at::Tensor q, at::Tensor k, at::Tensor v,
                                c10::optional<at::Tensor> q_lens,
                                c10::optional<at::Tensor> kv_lens,
                                double scale, bool causal) {
+  c10::OptionalDeviceGuard guard(at::device_of(q));
+  capture_check({q, k, v});
   if (at::GradMode::is_enabled() &&
       (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return AttentionRecompute::apply(q, k, v, q_lens, kv_lens, scale, causal);
@@ -524,6 +549,8 @@ std::vector<at::Tensor> qk_norm_rope_grad(
     c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cos,
     c10::optional<at::Tensor> sin, c10::optional<at::Tensor> pos, double eps,
     bool interleaved) {
+  c10::OptionalDeviceGuard guard(at::device_of(q));
+  capture_check({q, k, plain(wq), plain(wk)});
   bool w = wq.has_value() && wk.has_value() &&
            (wq->requires_grad() || wk->requires_grad());
   if (at::GradMode::is_enabled() &&
@@ -554,6 +581,7 @@ void bind_transformer(pybind11::module_& m) {
         py::arg("dout"), py::arg("q_lens"), py::arg("kv_lens"),
         py::arg("scale"), py::arg("causal"),
         py::arg("dv_out") = py::none());
+  m.def("capture_check", &capture_check);
   // differentiable forms
   m.def("attention_recompute", &attention_recompute, py::arg("q"),
         py::arg("k"), py::arg("v"), py::arg("q_lens"), py::arg("kv_lens"),

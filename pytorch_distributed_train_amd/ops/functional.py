@@ -987,7 +987,9 @@ def attention_recompute(q, k, v, scale: float | None = None,
     causal: query i sees keys up to i + kv_len - q_len, so the last query
     sees the last key. A query that sees none gives 0.
     GPU (csrc/attn_recompute.hip): bf16 and fp16, hd a multiple of 8 up to
-    128; results do not depend on timing; no gradient of the gradient.
+    128; results do not depend on timing; no gradient of the gradient. A
+    captured forward that needs gradients is refused while another graph of
+    the same leaves, made on the default stream, is alive.
     In fp16, gradients need a loss scale that keeps dS in its range, as the
     fp16 training path has."""
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape \
@@ -1254,6 +1256,7 @@ def attention_qkv_rope(qkv2d, q_weight, k_weight, cos, sin, b: int, s: int,
     if scale is None:
         scale = hd ** -0.5
     if qkv2d.is_cuda:
+        ext().capture_check([qkv2d, q_weight, k_weight])
         return AttentionQKVRopeFn.apply(qkv2d.contiguous(), q_weight,
                                         k_weight, cos, sin, b, s, h, hd,
                                         scale, causal, eps, gslot_q, gslot_k)

@@ -447,3 +447,36 @@ def test_one_gradient_of_several():
     with torch.inference_mode():
         assert torch.equal(OF.attention_recompute(q, k, v, causal=True),
                            want[0])
+
+
+@gpu
+def test_capture_beside_a_living_graph_is_refused():
+    """The capture's backward would end the process: refused in the forward;
+    once the other graph is gone it works."""
+    q, k, v, do = _inputs("cuda", torch.bfloat16, 1, 70, 70, 2, 2, 64)
+    leaf = q.clone().requires_grad_(True)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    alive = [OF.attention_recompute(leaf, k, v),
+             OF.qk_norm_rope(q, k, w, w.detach())]
+    for f in (lambda: OF.attention_recompute(leaf, k, v),
+              lambda: OF.qk_norm_rope(q, k, w, w.detach())):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="delete it first"):
+            with torch.cuda.graph(graph):
+                f()
+        torch.cuda.synchronize()
+        with torch.no_grad():  # no gradient: no objection
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                f()
+    want = torch.autograd.grad(alive[0], leaf, do)[0]
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(OF.attention_recompute(leaf, k, v), leaf,
+                                  do)[0]
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)

@@ -151,13 +151,14 @@ def _trainer(**kw):
 
 @gpu
 def test_trainer_steps_eager_and_captured():
-    """Three warm-up steps and four replays do what seven eager steps do,
-    with eager work between the replays."""
+    """An eager step, three warm-up steps and four replays do what eight
+    eager steps do, with eager work between the replays."""
     x = torch.randn(4, 3, 224, 224, device="cuda")
     y = torch.randint(0, 1000, (4,), device="cuda")
     a, b = _trainer(), _trainer()
     for t in (a, b):
         t.model.train()
+        t.train_step(x, y)
     assert a.enable_hip_graph(x, y)
     for _ in range(3):
         b.train_step(x, y)

@@ -1323,10 +1323,11 @@ struct Plan {
   // free: no causal mask and no lengths
   Plan(long b, long sq, long sk, long hk, long g, long hd, bool free) {
     long bh = b * hk, rows = sq * g;
-    // one block a head has to fill the chip. Sequences of few keys take D
-    // from P and dP, which only the two-pass backward does.
+    // One block a head has to fill the chip, or be short: 4 x 65 tokens of 3
+    // heads 10 against 15 us, but 8 x 197 of 12 26 against 24. Sequences of
+    // few keys take D from P and dP, which only the two-pass backward does.
     whole = free && hd <= 64 && sk > 64 && sk <= 256 && rows <= 256 &&
-            bh >= 256;
+            (bh >= 256 || (sk <= 128 && rows <= 128));
     long rblk = bh * ((rows + 127) / 128), kblk = bh * ((sk + 127) / 128);
     // two of its blocks a CU: 47 against 51 us at 1536 heads of 197 tokens,
     // and no gain below
@@ -1361,8 +1362,12 @@ struct Plan {
   }
 };
 
+// D of every row at the start of backward's workspace, the parts 16-byte
+// aligned behind it
+long delta_floats(long rows) { return (rows + 3) / 4 * 4; }
+
 template <typename T, int HDT>
-void launch(const Args& a, int bwd, float* ws, hipStream_t s) {
+void launch(Args a, int bwd, float* ws, hipStream_t s) {
   int rblk = (a.sq * a.g + 127) / 128, kblk = (a.sk + 127) / 128;
   int bh = a.b * a.hk, rblk256 = (a.sq * a.g + 255) / 256;
   Plan p(a.b, a.sq, a.sk, a.hk, a.g, a.hd,
@@ -1399,6 +1404,8 @@ void launch(const Args& a, int bwd, float* ws, hipStream_t s) {
     }
   long nq = (long)a.b * a.sq * a.hk * a.g * a.hd;
   long nk = (long)a.b * a.sk * a.hk * a.hd;
+  a.delta = ws;
+  ws += delta_floats(nq / a.hd);
   if (rblk) {
     attn_rc_dq_k<T, HDT><<<bh * rblk * p.dq, 256, 0, s>>>(a, rblk, p.dq, ws);
     if (p.dq > 1)
@@ -1418,24 +1425,25 @@ void launch(const Args& a, int bwd, float* ws, hipStream_t s) {
 
 extern "C" {
 
-// floats of workspace that forward or backward needs
+// floats of workspace that forward or backward needs; free: no causal mask
+// and no lengths
 long pdta_attn_recompute_ws(long b, long sq, long sk, long hk, long g,
-                            long hd, int bwd) {
-  Plan p(b, sq, sk, hk, g, hd, false);
+                            long hd, int free, int bwd) {
+  Plan p(b, sq, sk, hk, g, hd, free);
   long nq = b * sq * hk * g * hd, nk = b * sk * hk * hd;
   if (!bwd) return p.fwd > 1 ? p.fwd * (nq + nq / hd) : 0;
+  if (p.whole) return 0;
   long x = p.dq > 1 ? p.dq * nq : 0, y = p.dkv > 1 ? 2 * p.dkv * nk : 0;
-  return x > y ? x : y;
+  return delta_floats(nq / hd) + (x > y ? x : y);
 }
 
 // strides: q, k, v, dout, dv, each (b, s, head) in elements; multiples of 8,
 // all pointers 16-byte aligned, hd a multiple of 8 up to 128. lens null or [b].
 // Forward writes out and, unless null, lse; backward reads both and writes
-// delta, dq, dk, dv; either with pdta_attn_recompute_ws floats in ws. Grids must stay below 2^31 blocks and sq*g below 2^31.
+// dq, dk, dv; either with pdta_attn_recompute_ws floats in ws. Grids must stay below 2^31 blocks and sq*g below 2^31.
 void pdta_attn_recompute(const void* q, const void* k, const void* v,
                          const void* dout, const long* st, void* out,
-                         float* lse, float* delta, void* dq, void* dk,
-                         void* dv, const void* q_lens, const void* kv_lens,
+                         float* lse, void* dq, void* dk, void* dv, const void* q_lens, const void* kv_lens,
                          int lens64, int b, int sq, int sk, int hk, int g,
                          int hd, float scale, int causal, int bwd,
                          float* ws, int dt, hipStream_t s) {
@@ -1451,7 +1459,7 @@ void pdta_attn_recompute(const void* q, const void* k, const void* v,
   a.k = view(k, st + 3, false);
   a.v = view(v, st + 6, false);
   a.dout = view(dout, st + 9, true);
-  a.out = out, a.dq = dq, a.dk = dk, a.dv = dv, a.lse = lse, a.delta = delta;
+  a.out = out, a.dq = dq, a.dk = dk, a.dv = dv, a.lse = lse, a.delta = nullptr;
   a.vb = st[12], a.vs = st[13], a.vh = st[14];
   a.q_lens = q_lens, a.kv_lens = kv_lens, a.lens64 = lens64;
   a.b = b, a.sq = sq, a.sk = sk, a.hk = hk, a.g = g, a.hd = hd;

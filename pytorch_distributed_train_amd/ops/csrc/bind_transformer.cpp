@@ -24,11 +24,11 @@ void pdta_qknorm(const void* const*, const long*, const void* const*,
                  long, long, float, int, int, int, float*, float*, float*,
                  int, hipStream_t);
 void pdta_attn_recompute(const void*, const void*, const void*, const void*,
-                         const long*, void*, float*, float*, void*, void*,
-                         void*, const void*, const void*, int, int, int, int,
+                         const long*, void*, float*, void*, void*, void*,
+                         const void*, const void*, int, int, int, int,
                          int, int, int, float, int, int, float*, int,
                          hipStream_t);
-long pdta_attn_recompute_ws(long, long, long, long, long, long, int);
+long pdta_attn_recompute_ws(long, long, long, long, long, long, int, int);
 }
 
 namespace {
@@ -352,14 +352,15 @@ std::vector<at::Tensor> attn_recompute_fwd(
   attn_strides(k, st + 3);
   attn_strides(v, st + 6);
   if (out.numel()) {
+    bool free = !causal && !q_lens.has_value() && !kv_lens.has_value();
     long need =
-        pdta_attn_recompute_ws(n.b, n.sq, n.sk, n.hk, g, n.hd, 0);
+        pdta_attn_recompute_ws(n.b, n.sq, n.sk, n.hk, g, n.hd, free, 0);
     at::Tensor ws;
     if (need) ws = at::empty({need}, lse.options());
     pdta_attn_recompute(q.data_ptr(), k.data_ptr(), v.data_ptr(), nullptr,
                         st, out.data_ptr(),
                         want_lse ? lse.data_ptr<float>() : nullptr, nullptr,
-                        nullptr, nullptr, nullptr, len_ptr(q_lens),
+                        nullptr, nullptr, len_ptr(q_lens),
                         len_ptr(kv_lens), lens_wide(q_lens, kv_lens), n.b,
                         n.sq, n.sk, n.hk, g, n.hd, (float)scale, causal, 0,
                         need ? ws.data_ptr<float>() : nullptr, dt_of(q),
@@ -399,10 +400,10 @@ std::vector<at::Tensor> attn_recompute_bwd(
                   dv.sizes() == dk.sizes() &&
                   (dv.numel() == 0 || (dv.stride(3) == 1 && rows8(dv))),
               "dv_out must be like v, with aligned rows");
-  auto delta = at::empty_like(lse);
-  auto ws = at::empty(
-      {pdta_attn_recompute_ws(n.b, n.sq, n.sk, n.hk, g, n.hd, 1)},
-      lse.options());
+  bool free = !causal && !q_lens.has_value() && !kv_lens.has_value();
+  long need = pdta_attn_recompute_ws(n.b, n.sq, n.sk, n.hk, g, n.hd, free, 1);
+  at::Tensor ws;
+  if (need) ws = at::empty({need}, lse.options());
   long st[15];
   attn_strides(q, st);
   attn_strides(k, st + 3);
@@ -412,12 +413,12 @@ std::vector<at::Tensor> attn_recompute_bwd(
   if (dq.numel() || dk.numel()) {
     pdta_attn_recompute(q.data_ptr(), k.data_ptr(), v.data_ptr(),
                         dout.data_ptr(), st, out.data_ptr(),
-                        lse.data_ptr<float>(), delta.data_ptr<float>(),
-                        dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                        len_ptr(q_lens), len_ptr(kv_lens),
+                        lse.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
+                        dv.data_ptr(), len_ptr(q_lens), len_ptr(kv_lens),
                         lens_wide(q_lens, kv_lens), n.b, n.sq, n.sk, n.hk, g,
-                        n.hd, (float)scale, causal, 1, ws.data_ptr<float>(),
-                        dt_of(q), cur_stream());
+                        n.hd, (float)scale, causal, 1,
+                        need ? ws.data_ptr<float>() : nullptr, dt_of(q),
+                        cur_stream());
     launched("attn_recompute_bwd");
   }
   return {dq, dk, dv};

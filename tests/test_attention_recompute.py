@@ -150,6 +150,8 @@ CASES = [
     (128, 70, 130, 6, 2, 40, False, None, None),
     (256, 33, 256, 1, 1, 64, False, None, None),
     (300, 1, 65, 3, 1, 8, False, None, None),
+    (2, 128, 128, 2, 2, 64, False, None, None),   # ... and few short ones
+    (1, 40, 100, 6, 2, 48, False, None, None),
     # few rows against many keys, which are dealt out and joined
     (2, 1, 1000, 3, 3, 64, False, None, [0, 999]),
     (4, 3, 900, 6, 2, 96, True, [3, 0, 2, 1], [900, 5, 0, 513]),
@@ -341,7 +343,7 @@ def test_scale_and_empty():
     q, k, v, do = _inputs("cuda", torch.float16, 1, 50, 60, 2, 2, 64)
     want = _oracle(q, k, v, do, 0.31, False, None, None)
     _check(_run(q, k, v, do, scale=0.31), *want)
-    for b, sq, sk in ((0, 5, 5), (2, 0, 5), (2, 5, 0)):
+    for b, sq, sk in ((0, 5, 5), (2, 0, 5), (2, 5, 0), (2, 0, 100)):
         x = _inputs("cuda", torch.float16, b, sq, sk, 2, 1, 64)
         for u, w in zip(_run(*x), (x[0], x[0], x[1], x[2])):
             assert u.shape == w.shape and bool((u == 0).all())

@@ -49,6 +49,8 @@
 // bits for the latter, the bytes between groups set the others apart for the
 // former, and the way from row to row + 16 stays a constant. Conflicts took
 // 16 to 20% of all cycles at heads of 128 when perm alone did this.
+#include <cfloat>
+
 #include "common.h"
 
 namespace {
@@ -414,7 +416,7 @@ struct Running {
   f32x16 acc[G::DT];
   float c, far;
   DEV_INLINE explicit Running(float scale) : c(scale * kLog2e) {
-    far = 8.f / c;
+    far = fminf(8.f / c, FLT_MAX);  // top + far starts at -inf, not NaN
 #pragma unroll
     for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
   }
@@ -892,9 +894,8 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk,
 // blocks a CU; two: 490), 830 at 128; 16384 causal tokens, 16/2 heads of 128:
 // 2.1 ms.
 template <typename T, int HDT>
-__global__ __launch_bounds__(256, HDT == 64 ? 3 : 2) void attn_rc_dkv_k(Args a, int nblk,
-                                                        int nsplit,
-                                                        float* part) {
+__global__ __launch_bounds__(256, HDT == 64 ? 3 : 2) void attn_rc_dkv_k(
+    Args a, int nblk, int nsplit, float* part) {
   using G = Geo<HDT>;
   constexpr bool VLDS = HDT > 64;
   constexpr int RT = VLDS ? 32 : 64;
@@ -1055,7 +1056,8 @@ __global__ __launch_bounds__(256, HDT == 64 ? 3 : 2) void attn_rc_dkv_k(Args a, 
 // took 158 us at 1536 heads of 197 tokens, this one 120; the two kernels above
 // 163). dK and dV gather in registers as
 // in attn_rc_dkv_k. dQ needs all keys of a row: the waves put dS (16 bits,
-// which it has as an operand anyway) to LDS, and after a barrier each takes 16 columns of dQ's 32 rows over all keys, in 16x16x32 products.
+// which it has as an operand anyway) to LDS, and after a barrier each takes 16
+// columns of dQ's 32 rows over all keys, in 16x16x32 products.
 // dS lies by key, 32 rows or 64 bytes each, with its 8-byte pieces moved
 // about (ds_at) so that 32 keys' writes and the transposing reads' 8 keys x
 // 32 bytes meet distinct banks.
@@ -1174,14 +1176,11 @@ __global__ __launch_bounds__(256, 2) void attn_rc_bwd_short_k(Args a) {
       for (int ks = 0; ks < 4; ++ks)
         sc = Op<T>::mfma(frag_row<64>(qt, 0, ks, lane),
                          frag_row<64>(kall, grp * 32, ks, lane), sc);
-      // keeps the operands of one product at a time in registers: spilled
-      // ones would have to wait for the tile's loads
-      
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
         dp = Op<T>::mfma(frag_row<64>(dt, 0, ks, lane), vf[n][ks], dp);
-      
-      // the products' operands leave the registers first
+      // the products' operands leave the registers first: spilled ones would
+      // have to wait for the tile's loads
       __builtin_amdgcn_sched_barrier(0);
       unsigned p[8], d[8];
 #pragma unroll
@@ -1440,11 +1439,12 @@ long pdta_attn_recompute_ws(long b, long sq, long sk, long hk, long g,
 // strides: q, k, v, dout, dv, each (b, s, head) in elements; multiples of 8,
 // all pointers 16-byte aligned, hd a multiple of 8 up to 128. lens null or [b].
 // Forward writes out and, unless null, lse; backward reads both and writes
-// dq, dk, dv; either with pdta_attn_recompute_ws floats in ws. Grids must stay below 2^31 blocks and sq*g below 2^31.
+// dq, dk, dv; either with pdta_attn_recompute_ws floats in ws. Grids must stay
+// below 2^32 threads and sq*g below 2^31.
 void pdta_attn_recompute(const void* q, const void* k, const void* v,
                          const void* dout, const long* st, void* out,
-                         float* lse, void* dq, void* dk, void* dv, const void* q_lens, const void* kv_lens,
-                         int lens64, int b, int sq, int sk, int hk, int g,
+                         float* lse, void* dq, void* dk, void* dv,
+                         const void* q_lens, const void* kv_lens, int lens64, int b, int sq, int sk, int hk, int g,
                          int hd, float scale, int causal, int bwd,
                          float* ws, int dt, hipStream_t s) {
   Args a;

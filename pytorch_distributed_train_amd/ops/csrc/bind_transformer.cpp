@@ -138,7 +138,8 @@ std::vector<at::Tensor> qk_norm_rope(
               "q and k must be [b, s, heads, hd], alike but for the heads");
   long b = q.size(0), s = q.size(1), hd = q.size(3);
   TORCH_CHECK(hd >= 1 && hd <= 256, "head size must be 1 to 256, is ", hd);
-  TORCH_CHECK(b * s < (1l << 31) - 65536 && q.size(2) + k.size(2) < 65536,
+  // the forward has a wave a token; a grid holds 2^32 threads
+  TORCH_CHECK(b * s < (1l << 26) - 4 && q.size(2) + k.size(2) < 65536,
               "too many rows");
   bool bwd = dq.has_value();
   TORCH_CHECK(bwd == dk.has_value(), "dq and dk come together");
@@ -297,9 +298,9 @@ AttnShape attn_check(const at::Tensor& q, const at::Tensor& k,
                 "multiples of 8");
   }
   long g = n.hk ? n.h / n.hk : 1;
+  // blocks of 256 threads for 128 rows or keys; a grid holds 2^32 threads
   TORCH_CHECK((n.sq + n.sk + 1024) * g < (1l << 31) &&
-                  n.b * n.hk * ((n.sq * g + n.sk) / 128 + 2) * 64 <
-                      (1l << 31),
+                  n.b * n.hk * ((n.sq * g + n.sk) / 128 + 2) < (1l << 24),
               "attention: too many rows");
   for (const auto* l : {&q_lens, &kv_lens})
     if (l->has_value()) {
@@ -427,7 +428,7 @@ std::vector<at::Tensor> attn_recompute_bwd(
 // ---- autograd -----------------------------------------------------------
 // The GPU path's autograd nodes are C++: the engine's device thread then runs
 // backward without taking the GIL. 4 x 65 tokens of 3 heads, forward and
-// backward: 92 us with Python nodes, 68 with these, 20 of it kernels.
+// backward: 92 us with Python nodes, 68 with these; now 64, 18 of it kernels.
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 

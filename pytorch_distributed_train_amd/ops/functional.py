@@ -982,8 +982,9 @@ def attention_recompute(q, k, v, scale: float | None = None,
     scale: positive, None for 1/sqrt(hd).
     q_lens, kv_lens: int32 or int64 [b], the sequences' lengths (None: sq,
     sk); cut to 0..sq, 0..sk. What lies behind them is never read; outputs
-    and gradients there are 0. Inside them v has to be finite: a probability
-    of 0 does not keep a NaN or an infinity in it from earlier queries.
+    and gradients there are 0. Inside them every element has to be finite: a
+    pair that the causal mask hides counts 0 times what it holds, which does
+    not keep a NaN or an infinity from the other rows of its tile.
     causal: query i sees keys up to i + kv_len - q_len, so the last query
     sees the last key. A query that sees none gives 0.
     GPU (csrc/attn_recompute.hip): bf16 and fp16, hd a multiple of 8 up to
@@ -1253,6 +1254,10 @@ def attention_qkv_rope(qkv2d, q_weight, k_weight, cos, sin, b: int, s: int,
     if qkv2d.shape != (b * s, 3 * h * hd):
         raise ValueError(f"qkv must be [{b * s}, {3 * h * hd}]: "
                          f"{tuple(qkv2d.shape)}")
+    if q_weight is None or k_weight is None:
+        raise ValueError("q_weight and k_weight must be given")
+    if any(t is not None and t.requires_grad for t in (cos, sin)):
+        raise ValueError("cos and sin have no gradient")
     if scale is None:
         scale = hd ** -0.5
     if qkv2d.is_cuda:

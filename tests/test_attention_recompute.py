@@ -482,3 +482,54 @@ def test_capture_beside_a_living_graph_is_refused():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+@gpu
+def test_smallest_scale_gives_the_mean():
+    """Scores so small that the reference point of the softmax could pass
+    fp32's range on the way: every key has the same weight, so an output is a
+    mean, rounded once (and P once more)."""
+    q, k, v, _ = _inputs("cuda", torch.bfloat16, 1, 70, 600, 2, 2, 64)
+    for rows in (70, 3):
+        y = OF.attention_recompute(q[:, :rows], k, v, scale=1e-40)
+        want = v.double().mean(1, keepdim=True)
+        tol = 2 * 2.0 ** -8 * v.double().abs().mean(1, keepdim=True)
+        assert bool(((y.double() - want).abs() <= tol).all()), rows
+
+
+@gpu
+def test_refuses_more_than_a_grid_holds():
+    # 129 rows and keys make 4 blocks at most by the check; no memory is
+    # touched, the batch is one row seen many times
+    q = torch.zeros(1, 129, 1, 8, device="cuda", dtype=torch.bfloat16)
+    q = q.expand(6 << 20, 129, 1, 8)
+    with pytest.raises(RuntimeError, match="too many rows"):
+        OF.attention_recompute(q, q, q)
+
+
+@gpu
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_under_activation_checkpointing(reentrant):
+    from torch.utils.checkpoint import checkpoint
+    q, k, v, do = _inputs("cuda", torch.bfloat16, 2, 150, 150, 4, 2, 64)
+    want = _run(q, k, v, do, causal=True)
+    leaves = [x.detach().clone().requires_grad_(True) for x in (q, k, v)]
+    out = checkpoint(
+        lambda *x: OF.attention_recompute(*x, causal=True), *leaves,
+        use_reentrant=reentrant)
+    out.backward(do)
+    for a, b in zip(want, (out, *(x.grad for x in leaves))):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_projection_form_refusals(dev):
+    x = torch.zeros(8, 3 * 2 * 16, device=dev, dtype=torch.bfloat16)
+    w = torch.ones(16, device=dev)
+    cos, sin = OF.rope_tables(8, 16, device=dev)
+    for a in ((x[:7], w, w, cos, sin), (x, None, None, cos, sin),
+              (x, w, None, cos, sin),
+              (x, w, w, cos.clone().requires_grad_(True), sin),
+              (x, w, w, cos[:3], sin[:3])):
+        with pytest.raises((ValueError, RuntimeError)):
+            OF.attention_qkv_rope(*a, 1, 8, 2, 16)

@@ -307,3 +307,12 @@ def test_tables_and_weights_of_any_stride(dev):
                           positions=odd(p))
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@gpu
+def test_refuses_more_than_a_grid_holds():
+    # one token seen many times: no memory is touched
+    q = torch.zeros(1, 1, 1, 8, device="cuda").expand(1 << 26, 1, 1, 8)
+    w = torch.ones(8, device="cuda")
+    with pytest.raises(RuntimeError, match="too many rows"):
+        OF.qk_norm_rope(q, q, w, w)

@@ -129,25 +129,111 @@ struct Seq {
   DEV_INLINE Seq(const Args& a, int bh) {
     batch = uniform(bh / a.hk);
     kvh = bh - batch * a.hk;
-    qlen = length_of(a.q_lens, a.lens64, batch, a.sq);
-    klen = length_of(a.kv_lens, a.lens64, batch, a.sk);
+    set(a, length_of(a.q_lens, a.lens64, batch, a.sq),
+        length_of(a.kv_lens, a.lens64, batch, a.sk));
+  }
+  DEV_INLINE Seq(const Args& a, int batch_, int kvh_, int q, int k)
+      : batch(batch_), kvh(kvh_) {
+    set(a, q, k);
+  }
+  DEV_INLINE void set(const Args& a, int q, int k) {
+    qlen = q, klen = k;
     off = klen - qlen;
     rows = qlen * a.g;
   }
 };
 
-// Block index -> sequence and head, block of it, and part. Causal: all heads'
-// longest blocks first (LAST: high indexes are long). Else 8 heads at a time
-// (also with lengths: the longest blocks of all sequences first put long
-// blocks together on a CU and took 20% more).
-// Either way a head's blocks are 8 (or bh) apart, and as the hardware deals
+template <int CTRL, int ROWS>
+DEV_INLINE int dpp_add(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+// running sum over the wave's lanes
+DEV_INLINE int wave_scan(int x) {
+  x = dpp_add<0x111, 0xf>(x);  // from 1, 2, 4, 8 lanes before, in rows of 16
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);  // a row's last lane to the odd rows
+  return dpp_add<0x143, 0xc>(x);  // lane 31 to the upper half
+}
+
+// Blocks of sequences with lengths, longest first: block index -> block of
+// its head, sequence and head. KEYS: blocks of keys that run over the rows;
+// else of rows over the keys. Only the blocks in front of the sequence's end
+// have work; the others come last. Blocks go to the 8 dies in turn and there
+// to one CU after the other, two each; so a head's blocks stay on a die, and
+// the first 32 go there from short to long, so that the long ones share their
+// CU with the shortest of the next 32. 16 sequences of 0 to 777 tokens, 10
+// heads of 80: forward 34 us, dQ 43, dK/dV 53; in the order of the batch 40,
+// 49, 66. A block spends 1.4 us here; the longest run 20.
+// Lane l ranks sequence l (b <= 64) and then places head die + 8 l; heads are
+// a multiple of 8 up to 512.
+template <bool KEYS, int BLOCK>
+DEV_INLINE Seq by_length(const Args& a, int nblk, int nsplit, int* bh,
+                         int* blk) {
+  int lane = threadIdx.x & 63, die = blockIdx.x & 7, at = blockIdx.x >> 3;
+  bool in = lane < a.b;
+  int ql = in ? length_of(a.q_lens, a.lens64, lane, a.sq) : -1;
+  int kl = in ? length_of(a.kv_lens, a.lens64, lane, a.sk) : -1;
+  int n = KEYS ? ql : kl, rank = 0;
+  // lanes from a.b on hold -1: they are not counted
+  for (int j = 0; j < a.b; j += 4)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      rank += __builtin_amdgcn_readlane(n, j + i) >= n + (j + i >= lane);
+  int live = ((KEYS ? kl : ql * a.g) + BLOCK - 1) / BLOCK * nsplit;
+  live = n > 0 ? live : 0;
+  // by rank, then by head
+  int x = __builtin_amdgcn_ds_permute((in ? rank : lane) * 4,
+                                      live << 6 | lane);
+  int j = (die + 8 * lane) / a.hk;
+  x = __builtin_amdgcn_ds_bpermute((j & 63) * 4, x);
+  int seq = x & 63;
+  live = j < a.b ? x >> 6 : 0;
+  int upto = wave_scan(live);
+  int total = __builtin_amdgcn_readlane(upto, 63);
+  if (at < total) {
+    int first = total < 32 ? total : 32;
+    if (at < first) at = first - 1 - at;
+  } else {
+    // past the live ones: head by head the blocks behind them
+    at -= total;
+    upto = nblk * (lane + 1) - upto;
+    live = nblk;
+  }
+  int to = __builtin_ctzll(__ballot(upto > at));
+  *blk = at - __builtin_amdgcn_readlane(upto - live, to);
+  seq = __builtin_amdgcn_readlane(seq, to);
+  int kvh = die + 8 * to - __builtin_amdgcn_readlane(j, to) * a.hk;
+  *bh = seq * a.hk + kvh;
+  return Seq(a, seq, kvh, __builtin_amdgcn_readlane(ql, seq),
+             __builtin_amdgcn_readlane(kl, seq));
+}
+
+// Block index -> block and part, sequence and head. Causal: all heads' longest
+// blocks first. With lengths: by_length. Else 8 heads at a time. In each case
+// a head's blocks are a multiple of 8 (or bh) apart, and as the hardware deals
 // blocks out to its 8 dies in turn, they meet in one die's L2.
-DEV_INLINE void place(const Args& a, int nblk, bool last, int* bh, int* blk) {
+template <bool KEYS, int BLOCK = 128>
+DEV_INLINE Seq place(const Args& a, int nblk, int nsplit, int* bh, int* blk,
+                     int* split) {
   int heads = a.b * a.hk, i = blockIdx.x;
+  nblk *= nsplit;
+  auto parted = [&] {
+    int x = *blk;
+    *blk = uniform(x / nsplit);
+    *split = x - *blk * nsplit;
+  };
+  if (!a.causal && (KEYS ? a.q_lens : a.kv_lens) && a.b <= 64 &&
+      heads <= 512 && heads % 8 == 0) {
+    Seq s = by_length<KEYS, BLOCK>(a, nblk, nsplit, bh, blk);
+    parted();
+    return s;
+  }
   if (a.causal) {
     *blk = uniform(i / heads);
     *bh = i - *blk * heads;
-    if (last) *blk = nblk - 1 - *blk;
+    if (!KEYS) *blk = nblk - 1 - *blk;
   } else {
     int grp = uniform(i / (8 * nblk)), w = i - grp * 8 * nblk;
     int n = heads - grp * 8;
@@ -155,6 +241,17 @@ DEV_INLINE void place(const Args& a, int nblk, bool last, int* bh, int* blk) {
     *blk = uniform(w / n);
     *bh = grp * 8 + w - *blk * n;
   }
+  parted();
+  return Seq(a, *bh);
+}
+
+// zeros to n pieces of 16 * chunks bytes, 32 chunks at most
+template <typename F>
+DEV_INLINE void clear(int n, int chunks, F piece) {
+  int c = threadIdx.x & 31;
+  if (c >= chunks) return;
+  for (int i = threadIdx.x >> 5; i < n; i += blockDim.x >> 5)
+    reinterpret_cast<uint4*>(piece(i))[c] = {0, 0, 0, 0};
 }
 
 template <int HDT> struct Geo {
@@ -508,6 +605,27 @@ struct Running {
   }
 };
 
+// forward of a block of n packed rows from r0 on that see no key, or none of
+// part `at`'s
+DEV_INLINE void no_keys(const Args& a, const Seq& s, int bh, int r0, int n,
+                        int parts, int at, float* part) {
+  int all = a.sq * a.g;
+  n = all - r0 < n ? all - r0 : n;
+  long r = (long)bh * all + r0, rows = (long)a.b * a.hk * all;
+  float* lse = parts == 1 ? a.lse + r : part + parts * rows * a.hd +
+                                            at * rows + r;
+  if ((parts > 1 || a.lse) && (int)threadIdx.x < n)
+    lse[threadIdx.x] = INFINITY;
+  if (parts > 1) return;  // no output is read then
+  clear(n, a.hd / 8, [&](int i) {
+    int pos = (int)mdiv(r0 + i, a.g_mul, a.g_shift);
+    return reinterpret_cast<short*>(a.out) +
+           (((long)s.batch * a.sq + pos) * a.hk * a.g + s.kvh * a.g + r0 + i -
+            pos * a.g) *
+               a.hd;
+  });
+}
+
 // ---- forward: a block has 128 packed rows, a wave 32 ----------------------
 // nsplit > 1: the keys' tiles go in runs of `per` to that many blocks, whose
 // results a last kernel joins. 4 x 4096 tokens x 12 heads: 250 us at heads of
@@ -523,19 +641,8 @@ __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk,
   LDS_BUFFER(v1, G::bytes(TILE));
   int lane = threadIdx.x & 63;
   int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int bh, blk;
-  place(a, nblk * nsplit, true, &bh, &blk);
-  int split = blk;
-  blk = uniform(blk / nsplit);
-  split -= blk * nsplit;
-  Seq s(a, bh);
-  Row row(a, s, blk * 128 + wave * 32 + (lane & 31));
-  Stream<HDT, TILE, false> kin(a, a.k, s, lane), vin(a, a.v, s, lane);
-  s16x8 qf[G::KS];
-  keep<HDT>(a,
-            reinterpret_cast<const char*>(a.q.p) +
-                2 * (s.batch * a.q.sb + row.pos * a.q.ss + row.head * a.q.sh),
-            row.valid, lane, qf);
+  int bh, blk, split;
+  Seq s = place<false>(a, nblk, nsplit, &bh, &blk, &split);
   // keys that any row of the block sees: the last row's, or none
   int last = (blk * 128 + 127) / a.g;
   last = last < s.qlen ? last : s.qlen - 1;
@@ -544,6 +651,17 @@ __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk,
   int ntile = end > 0 ? (end + TILE - 1) / TILE : 0;
   int first = split * per;
   if (nsplit > 1 && ntile > first + per) ntile = first + per;
+  if (first >= ntile) {
+    no_keys(a, s, bh, blk * 128, 128, nsplit, split, part);
+    return;
+  }
+  Row row(a, s, blk * 128 + wave * 32 + (lane & 31));
+  Stream<HDT, TILE, false> kin(a, a.k, s, lane), vin(a, a.v, s, lane);
+  s16x8 qf[G::KS];
+  keep<HDT>(a,
+            reinterpret_cast<const char*>(a.q.p) +
+                2 * (s.batch * a.q.sb + row.pos * a.q.ss + row.head * a.q.sh),
+            row.valid, lane, qf);
   int wlo = wave_min(row.lim), whi = wave_max(row.valid ? row.lim : 0);
   Running<T, HDT> run(a.scale);
   auto load = [&](int t, char* kd, char* vd) {
@@ -579,11 +697,14 @@ __global__ __launch_bounds__(512, 4) void attn_rc_fwd_short_k(Args a,
   LDS_BUFFER(vall, G::bytes(256));
   int lane = threadIdx.x & 63;
   int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int bh, blk;
-  place(a, nblk, true, &bh, &blk);
-  Seq s(a, bh);
+  int bh, blk, split;
+  Seq s = place<false, 256>(a, nblk, 1, &bh, &blk, &split);
   Stream<64, 64, false, 8> kin(a, a.k, s, lane), vin(a, a.v, s, lane);
   int end = blk * 256 < s.rows ? s.klen : 0;
+  if (end == 0) {
+    no_keys(a, s, bh, blk * 256, 256, 1, 0, nullptr);
+    return;
+  }
   int ntile = (end + 63) / 64;
   for (int t = 0; t < ntile; ++t) {
     kin.load(a, t * 64, s.klen, kall + G::bytes(64) * t, wave, lane);
@@ -752,25 +873,40 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk,
   LDS_BUFFER(v1, G::bytes(TILE));
   int lane = threadIdx.x & 63, h = lane >> 5;
   int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int bh, blk;
-  place(a, nblk * nsplit, true, &bh, &blk);
-  int split = blk;
-  blk = uniform(blk / nsplit);
-  split -= blk * nsplit;
-  Seq s(a, bh);
-  Row row(a, s, blk * 128 + wave * 32 + (lane & 31));
-  Stream<HDT, TILE, false> kin(a, a.k, s, lane), vin(a, a.v, s, lane);
+  int bh, blk, split;
+  Seq s = place<false>(a, nblk, nsplit, &bh, &blk, &split);
   int last = (blk * 128 + 127) / a.g;
   last = last < s.qlen ? last : s.qlen - 1;
   int end = blk * 128 < s.rows ? s.klen : 0;
   if (a.causal && last + s.off + 1 < end) end = last + s.off + 1;
   int ntile = end > 0 ? (end + TILE - 1) / TILE : 0;
+  if (split >= ntile) {  // nothing to see, or no tile for this part
+    int all = a.sq * a.g, n = all - blk * 128 < 128 ? all - blk * 128 : 128;
+    if (split == 0 && (int)threadIdx.x < n)
+      a.delta[(long)bh * all + blk * 128 + threadIdx.x] = 0.f;
+    auto at = [&](int i) {
+      int r = blk * 128 + i, pos = (int)mdiv(r, a.g_mul, a.g_shift);
+      return (((long)s.batch * a.sq + pos) * a.hk * a.g + s.kvh * a.g + r -
+              pos * a.g) *
+             a.hd;
+    };
+    if (nsplit == 1)
+      clear(n, a.hd / 8,
+            [&](int i) { return reinterpret_cast<T*>(a.dq) + at(i); });
+    else
+      clear(n, a.hd / 4, [&](int i) {
+        return part + (long)split * a.b * a.sq * a.hk * a.g * a.hd + at(i);
+      });
+    return;
+  }
+  Row row(a, s, blk * 128 + wave * 32 + (lane & 31));
+  Stream<HDT, TILE, false> kin(a, a.k, s, lane), vin(a, a.v, s, lane);
   int wlo = wave_min(row.lim), whi = wave_max(row.valid ? row.lim : 0);
   auto load = [&](int t, char* kd, char* vd) {
     kin.load(a, t * TILE, s.klen, kd, wave, lane);
     vin.load(a, t * TILE, s.klen, vd, wave, lane);
   };
-  if (split < ntile) load(split, k0, v0);
+  load(split, k0, v0);
   s16x8 qf[G::KS], df[G::KS];
   keep<HDT>(a,
             reinterpret_cast<const char*>(a.dout.p) +
@@ -846,7 +982,7 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk,
     }
   };
   staged();
-  if (split == 0 && ntile > 0 && wlo <= TILE) {
+  if (split == 0 && wlo <= TILE) {
     float d = 0.f;
 #pragma unroll 1
     for (int u = 0; u < 2; ++u) {
@@ -908,12 +1044,34 @@ __global__ __launch_bounds__(256, HDT == 64 ? 3 : 2) void attn_rc_dkv_k(
   LDS_BUFFER(vkeep, VLDS ? G::bytes(128) : 16);
   int lane = threadIdx.x & 63, h = lane >> 5;
   int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int bh, blk;
-  place(a, nblk * nsplit, false, &bh, &blk);
-  int split = blk;
-  blk = uniform(blk / nsplit);
-  split -= blk * nsplit;
-  Seq s(a, bh);
+  int bh, blk, split;
+  Seq s = place<true>(a, nblk, nsplit, &bh, &blk, &split);
+  int first = 0;
+  if (a.causal && blk * 128 > s.off) first = (blk * 128 - s.off) * a.g;
+  first &= ~(RT - 1);
+  int ntile = 0;
+  if (blk * 128 < s.klen && first < s.rows)
+    ntile = (s.rows - first + RT - 1) / RT;
+  if (split >= ntile) {  // no row sees these keys, or no tile for this part
+    int n = a.sk - blk * 128 < 128 ? a.sk - blk * 128 : 128;
+    auto at = [&](int i) {
+      return (((long)s.batch * a.sk + blk * 128 + i) * a.hk + s.kvh) * a.hd;
+    };
+    if (nsplit == 1) {
+      clear(n, a.hd / 8,
+            [&](int i) { return reinterpret_cast<T*>(a.dk) + at(i); });
+      clear(n, a.hd / 8, [&](int i) {
+        return reinterpret_cast<T*>(a.dv) + s.batch * a.vb +
+               (blk * 128 + i) * a.vs + s.kvh * a.vh;
+      });
+    } else {
+      long all = (long)a.b * a.sk * a.hk * a.hd;
+      float* out = part + 2 * split * all;
+      clear(n, a.hd / 4, [&](int i) { return out + at(i); });
+      clear(n, a.hd / 4, [&](int i) { return out + all + at(i); });
+    }
+    return;
+  }
   int key = blk * 128 + wave * 32 + (lane & 31);
   bool valid = key < s.klen;
   Stream<HDT, RT, true> qin(a, a.q, s, lane), din(a, a.dout, s, lane);
@@ -926,12 +1084,6 @@ __global__ __launch_bounds__(256, HDT == 64 ? 3 : 2) void attn_rc_dkv_k(
   // rows from `lo` on see this lane's key
   int lo = 0;
   if (a.causal) lo = key > s.off ? (key - s.off) * a.g : 0;
-  int first = 0;
-  if (a.causal && blk * 128 > s.off) first = (blk * 128 - s.off) * a.g;
-  first &= ~(RT - 1);
-  int ntile = 0;
-  if (blk * 128 < s.klen && first < s.rows)
-    ntile = (s.rows - first + RT - 1) / RT;
   int wlo = wave_min(lo), whi = wave_max(valid ? lo : 0);
   bool wlive = wave_max(valid) != 0;
 
@@ -948,13 +1100,11 @@ __global__ __launch_bounds__(256, HDT == 64 ? 3 : 2) void attn_rc_dkv_k(
     }
   };
   s16x8 kf[G::KS], vf[VLDS ? 1 : G::KS];
-  if (split < ntile) {
-    load(split, q0, d0, stat0);
-    if (VLDS) {
-      Stream<HDT, 128, false> vin(a, a.v, s, lane);
-      vin.quick = false;  // zeros past the head's end: dO has none there
-      vin.load(a, blk * 128, s.klen, vkeep, wave, lane);
-    }
+  load(split, q0, d0, stat0);
+  if (VLDS) {
+    Stream<HDT, 128, false> vin(a, a.v, s, lane);
+    vin.quick = false;  // zeros past the head's end: dO has none there
+    vin.load(a, blk * 128, s.klen, vkeep, wave, lane);
   }
   keep<HDT>(a, kb + 2 * (key * a.k.ss), valid, lane, kf);
   if (!VLDS) keep<HDT>(a, vb + 2 * (key * a.v.ss), valid, lane, vf);

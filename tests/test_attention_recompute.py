@@ -533,3 +533,39 @@ def test_projection_form_refusals(dev):
               (x, w, w, cos[:3], sin[:3])):
         with pytest.raises((ValueError, RuntimeError)):
             OF.attention_qkv_rope(*a, 1, 8, 2, 16)
+
+
+def _lengths(n, most):
+    """n lengths over 0..most in no order, some alike, some past the ends."""
+    x = [(i * 37) % (most + 1) for i in range(n)]
+    x[n // 2], x[n // 3], x[0] = most + 9, -4, most
+    return x
+
+
+@gpu
+@pytest.mark.parametrize("b,sq,sk,h,hk,hd,ql,kl", [
+    (16, 300, 300, 5, 5, 80, True, True),
+    (8, 300, 200, 4, 2, 64, True, False),     # lengths of one side
+    (8, 200, 300, 3, 1, 128, False, True),
+    (64, 150, 150, 8, 8, 64, True, True),     # as many as are put in order
+    (66, 140, 140, 4, 4, 72, True, True),     # more: in the batch's order
+    (3, 260, 260, 3, 3, 64, True, True),      # heads no multiple of 8
+    (4, 130, 1100, 2, 2, 64, True, True),     # keys dealt out and joined
+    (8, 1100, 300, 1, 1, 128, True, True),    # rows dealt out and joined
+    (8, 40, 1100, 12, 1, 64, True, True),
+    (2, 200, 200, 4, 4, 8, True, True),
+], ids=str)
+def test_lengths_in_any_order(b, sq, sk, h, hk, hd, ql, kl):
+    """Blocks of the longest sequences start first: each has to come up once,
+    those behind a sequence's end with zeros."""
+    q, k, v, do = _inputs("cuda", torch.float16, b, sq, sk, h, hk, hd)
+    ql = _lengths(b, sq) if ql else None
+    kl = _lengths(b, sk) if kl else None
+    if ql and kl and sq == sk:
+        kl = ql
+    want = _oracle(q, k, v, do, hd ** -0.5, False, ql, kl)
+    # NaN in the freed memory where the results will lie
+    stale = [torch.full_like(x, float("nan")) for x in (q, q, k, k)]
+    del stale
+    got = _run(q, k, v, do, q_lens=_t(ql, "cuda"), kv_lens=_t(kl, "cuda"))
+    _check(got, *want)

@@ -32,10 +32,10 @@
 // dS.
 //
 // What bounds it: 9 products of 2*hd flops a visible pair, where two (S and
-// dP again for dK, dV) are the price of no atomics. The two backward kernels
-// reach 1000 to 1150 TFLOP/s on long sequences with heads of 128, the
+// dP again for dK, dV) are the price of no atomics. On long sequences with
+// heads of 128 dQ reaches 1150 to 1250 TFLOP/s, dK/dV 1020 to 1100, the
 // forward 1030; a large matrix product reaches 1250. Heads of 64 have half
-// the products an exponential: 820 to 980. Splitting differently was slower:
+// the products an exponential: 800 to 1000. Splitting differently was slower:
 // scores one tile ahead of the softmax (more registers, fewer waves: 0 to
 // -25%), 32-key tiles with three blocks a CU (+4% long, -6% short).
 //
@@ -423,20 +423,26 @@ DEV_INLINE void keep(const Args& a, const char* row, bool valid, int lane,
 }
 
 // accumulators acc[DT] (lane: one row, d = 32*dt + 8*j + 4*h + 0..3) times m
-// to the row's memory, 8 bytes a piece
+// to the row's memory. A row's two lanes swap every second piece, so that each
+// stores 16 bytes.
 template <typename T, int DT>
 DEV_INLINE void put_row(T* row, const f32x16* acc, float m, int hd, int lane) {
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      int d = dt * 32 + j * 8 + (lane >> 5) * 4;
-      if (d < hd) {
-        uint2 v = {Op<T>::pack(acc[dt][4 * j] * m, acc[dt][4 * j + 1] * m),
-                   Op<T>::pack(acc[dt][4 * j + 2] * m,
-                               acc[dt][4 * j + 3] * m)};
-        *reinterpret_cast<uint2*>(row + d) = v;
+    for (int j = 0; j < 4; j += 2) {
+      unsigned v[4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int x = 4 * j + 2 * i, y = x + 4;
+        auto p = __builtin_amdgcn_permlane32_swap(
+            Op<T>::pack(acc[dt][x] * m, acc[dt][x + 1] * m),
+            Op<T>::pack(acc[dt][y] * m, acc[dt][y + 1] * m), false, false);
+        v[i] = p[0], v[i + 2] = p[1];
       }
+      int d = dt * 32 + (j + (lane >> 5)) * 8;
+      if (d < hd)
+        *reinterpret_cast<uint4*>(row + d) = {v[0], v[1], v[2], v[3]};
     }
 }
 
@@ -860,8 +866,9 @@ __global__ __launch_bounds__(256) void attn_rc_join_rows_k(Args a, int parts,
 
 // ---- backward 1: D, and dQ of 128 packed rows -----------------------------
 // nsplit > 1: the keys' tiles go to that many blocks in turn, whose fp32 sums
-// a last kernel adds. 4 x 4096 tokens x 12 heads: 320 us at heads of 64, 580
-// at 128; 16384 causal tokens, 16/2 heads of 128: 1.43 ms.
+// a last kernel adds. 4 x 4096 tokens x 12 heads: 308 us at heads of 64, 541
+// at 128; 16384 causal tokens, 16/2 heads of 128: 1.3 to 1.4 ms. dP's sums start
+// from -D, here and for dK, dV: 1 to 3% less than a subtraction behind them.
 template <typename T, int HDT>
 __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk,
                                                        int nsplit,
@@ -942,10 +949,11 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk,
   f32x16 acc[G::DT];
 #pragma unroll
   for (int i = 0; i < G::DT; ++i) acc[i] = kNone;
-  // P and dP of keys key0.. that lie at rows r0.. of the tiles
+  // P and dP plus `from` of keys key0.. that lie at rows r0.. of the tiles
   auto probs = [&](const char* kt, const char* vt, int r0, int key0,
-                   f32x16& sc, f32x16& dp) {
-    sc = dp = kNone;
+                   const f32x16& from, f32x16& sc, f32x16& dp) {
+    sc = kNone;
+    dp = from;
 #pragma unroll
     for (int ks = 0; ks < G::KS; ++ks) {
       sc = Op<T>::mfma(frag_row<HDT>(kt, r0, ks, lane), qf[ks], sc);
@@ -961,18 +969,18 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk,
     for (int i = 0; i < 16; ++i)
       sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], c, -lse));
   };
+  f32x16 less;  // -D: dP's products start from it
   auto step = [&](int t, const char* kt, const char* vt) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       int key0 = t * TILE + u * 32;
       if (key0 >= whi) return;
       f32x16 x, dp;
-      probs(kt, vt, u * 32, key0, x, dp);
+      probs(kt, vt, u * 32, key0, less, x, dp);
       unsigned p[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        p[i] = Op<T>::pack(x[2 * i] * (dp[2 * i] - delta),
-                           x[2 * i + 1] * (dp[2 * i + 1] - delta));
+        p[i] = Op<T>::pack(x[2 * i] * dp[2 * i], x[2 * i + 1] * dp[2 * i + 1]);
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -987,14 +995,16 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk,
 #pragma unroll 1
     for (int u = 0; u < 2; ++u) {
       f32x16 x, dp;
-      probs(k0, v0, u * 32, u * 32, x, dp);
+      probs(k0, v0, u * 32, u * 32, kNone, x, dp);
 #pragma unroll
       for (int i = 0; i < 16; ++i) d += x[i] * dp[i];
     }
     d += other_half(d);
     if (row.lim <= TILE) delta = row.valid ? d : 0.f;
   }
-  if (row.stored && h == 0 && split == 0) a.delta[lat] = delta;
+  if (row.stored && h == 0 && split == 0) a.delta[lat] = -delta;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) less[i] = -delta;
   for (int t = split; t < ntile; t += 2 * nsplit) {
     int t1 = t + nsplit, t2 = t1 + nsplit;
     if (t1 < ntile) load(t1, k1, v1);
@@ -1026,9 +1036,9 @@ __global__ __launch_bounds__(256, 2) void attn_rc_dq_k(Args a, int nblk,
 // With few key blocks the rows are dealt out to `nsplit` blocks in turn
 // (tile t to block t % nsplit), whose fp32 sums a last kernel adds; runs of
 // tiles instead, so that causal blocks are alike in length, took 1.4 to 1.8
-// times as long. 4 x 4096 tokens x 12 heads: 460 us at heads of 64 (three
-// blocks a CU; two: 490), 830 at 128; 16384 causal tokens, 16/2 heads of 128:
-// 2.1 ms.
+// times as long. 4 x 4096 tokens x 12 heads: 427 us at heads of 64 (three
+// blocks a CU; two took 6% more), 808 at 128; 16384 causal tokens, 16/2 heads
+// of 128: 2.0 to 2.1 ms.
 template <typename T, int HDT>
 __global__ __launch_bounds__(256, HDT == 64 ? 3 : 2) void attn_rc_dkv_k(
     Args a, int nblk, int nsplit, float* part) {
@@ -1039,10 +1049,10 @@ __global__ __launch_bounds__(256, HDT == 64 ? 3 : 2) void attn_rc_dkv_k(
   LDS_BUFFER(q1, G::bytes(RT));
   LDS_BUFFER(d0, G::bytes(RT));
   LDS_BUFFER(d1, G::bytes(RT));
-  LDS_BUFFER(stat0, 512);  // 64 rows' lse and D
+  LDS_BUFFER(stat0, 512);  // 64 rows' lse and -D
   LDS_BUFFER(stat1, 512);
   LDS_BUFFER(vkeep, VLDS ? G::bytes(128) : 16);
-  int lane = threadIdx.x & 63, h = lane >> 5;
+  int lane = threadIdx.x & 63;
   int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int bh, blk, split;
   Seq s = place<true>(a, nblk, nsplit, &bh, &blk, &split);
@@ -1117,11 +1127,19 @@ __global__ __launch_bounds__(256, HDT == 64 ? 3 : 2) void attn_rc_dkv_k(
     const float* ds = ls + 64;
     int ln = lane;  // some addresses are worked out anew, for registers
     asm volatile("" : "+v"(ln));
+    int h = ln >> 5;
 #pragma unroll
     for (int u = 0; u < RT / 32; ++u) {
       int r0 = first + t * RT + u * 32;
       if (!wlive || r0 + 32 <= wlo || r0 >= s.rows) continue;
-      f32x16 sc = kNone, dp = kNone;
+      f32x16 sc = kNone, dp;  // dP - D
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float4 d4 =
+            *reinterpret_cast<const float4*>(ds + u * 32 + j * 8 + h * 4);
+        dp[4 * j] = d4.x, dp[4 * j + 1] = d4.y;
+        dp[4 * j + 2] = d4.z, dp[4 * j + 3] = d4.w;
+      }
 #pragma unroll
       for (int ks = 0; ks < G::KS; ++ks) {
         sc = Op<T>::mfma(frag_row<HDT>(qt, u * 32, ks, lane), kf[ks], sc);
@@ -1141,9 +1159,7 @@ __global__ __launch_bounds__(256, HDT == 64 ? 3 : 2) void attn_rc_dkv_k(
       for (int j = 0; j < 4; ++j) {
         float4 l4 =
             *reinterpret_cast<const float4*>(ls + u * 32 + j * 8 + h * 4);
-        float4 d4 =
-            *reinterpret_cast<const float4*>(ds + u * 32 + j * 8 + h * 4);
-        const float *lp = &l4.x, *dl = &d4.x;
+        const float* lp = &l4.x;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float x = __builtin_amdgcn_exp2f(
@@ -1151,11 +1167,12 @@ __global__ __launch_bounds__(256, HDT == 64 ? 3 : 2) void attn_rc_dkv_k(
           float y = __builtin_amdgcn_exp2f(
               fmaf(sc[4 * j + 2 * i + 1], c, -lp[2 * i + 1]));
           p[2 * j + i] = Op<T>::pack(x, y);
-          d[2 * j + i] =
-              Op<T>::pack(x * (dp[4 * j + 2 * i] - dl[2 * i]),
-                          y * (dp[4 * j + 2 * i + 1] - dl[2 * i + 1]));
+          d[2 * j + i] = Op<T>::pack(x * dp[4 * j + 2 * i],
+                                     y * dp[4 * j + 2 * i + 1]);
         }
       }
+      // these products' operands are fetched only now: K or V went to scratch
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -1178,8 +1195,10 @@ __global__ __launch_bounds__(256, HDT == 64 ? 3 : 2) void attn_rc_dkv_k(
     step(t1, q1, d1, stat1);
     staged();
   }
+  asm volatile("" : "+v"(lane));  // worked out anew, for registers
+  key = blk * 128 + wave * 32 + (lane & 31);
   if (key >= a.sk) return;
-  if (!valid)
+  if (key >= s.klen)
 #pragma unroll
     for (int i = 0; i < G::DT; ++i) dk[i] = dv[i] = kNone;
   long at = (((long)s.batch * a.sk + key) * a.hk + s.kvh) * a.hd;
@@ -1203,7 +1222,7 @@ __global__ __launch_bounds__(256, HDT == 64 ? 3 : 2) void attn_rc_dkv_k(
 // rows 32 at a time, so S, dP and the exponentials are worked out once, and
 // q, k, v, out and dout are read once. Two blocks share a CU, so that one's
 // loads and barriers pass under the other's products (one block of 8 waves
-// took 158 us at 1536 heads of 197 tokens, this one 120; the two kernels above
+// took 158 us at 1536 heads of 197 tokens, this one 117; the two kernels above
 // 163). dK and dV gather in registers as
 // in attn_rc_dkv_k. dQ needs all keys of a row: the waves put dS (16 bits,
 // which it has as an operand anyway) to LDS, and after a barrier each takes 16
@@ -1511,7 +1530,7 @@ struct Plan {
   }
 };
 
-// D of every row at the start of backward's workspace, the parts 16-byte
+// -D of every row at the start of backward's workspace, the parts 16-byte
 // aligned behind it
 long delta_floats(long rows) { return (rows + 3) / 4 * 4; }
 

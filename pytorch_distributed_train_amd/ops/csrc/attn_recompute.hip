@@ -633,12 +633,13 @@ DEV_INLINE void no_keys(const Args& a, const Seq& s, int bh, int r0, int n,
 }
 
 // ---- forward: a block has 128 packed rows, a wave 32 ----------------------
-// nsplit > 1: the keys' tiles go in runs of `per` to that many blocks, whose
-// results a last kernel joins. 4 x 4096 tokens x 12 heads: 250 us at heads of
+// nsplit > 1: the keys' tiles go to that many blocks in turn, whose results a
+// last kernel joins (in runs, causal blocks were done at different times: 268
+// against 161 us for 16384 tokens of 2 heads of 128). 4 x 4096 tokens x 12 heads: 250 us at heads of
 // 64, 435 at 128; 16384 causal tokens, 16/2 heads of 128: 1.07 ms.
 template <typename T, int HDT>
 __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk,
-                                                        int nsplit, int per,
+                                                        int nsplit,
                                                         float* part) {
   using G = Geo<HDT>;
   LDS_BUFFER(k0, G::bytes(TILE));
@@ -655,9 +656,7 @@ __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk,
   int end = blk * 128 < s.rows ? s.klen : 0;
   if (a.causal && last + s.off + 1 < end) end = last + s.off + 1;
   int ntile = end > 0 ? (end + TILE - 1) / TILE : 0;
-  int first = split * per;
-  if (nsplit > 1 && ntile > first + per) ntile = first + per;
-  if (first >= ntile) {
+  if (split >= ntile) {
     no_keys(a, s, bh, blk * 128, 128, nsplit, split, part);
     return;
   }
@@ -678,15 +677,16 @@ __global__ __launch_bounds__(256, 2) void attn_rc_fwd_k(Args a, int nblk,
     if (t * TILE < whi)
       run.template step<2>(kt, vt, qf, t * TILE, row.lim, wlo, lane);
   };
-  if (first < ntile) load(first, k0, v0);
+  load(split, k0, v0);
   staged();
-  for (int t = first; t < ntile; t += 2) {
-    if (t + 1 < ntile) load(t + 1, k1, v1);
+  for (int t = split; t < ntile; t += 2 * nsplit) {
+    int t1 = t + nsplit, t2 = t1 + nsplit;
+    if (t1 < ntile) load(t1, k1, v1);
     step(t, k0, v0);
     staged();
-    if (t + 1 >= ntile) break;
-    if (t + 2 < ntile) load(t + 2, k0, v0);
-    step(t + 1, k1, v1);
+    if (t1 >= ntile) break;
+    if (t2 < ntile) load(t2, k0, v0);
+    step(t1, k1, v1);
     staged();
   }
   run.put(a, s, row, bh, nsplit, split, part, lane);
@@ -1483,19 +1483,20 @@ __global__ __launch_bounds__(256) void attn_rc_join_k(
 // How work is dealt out where there are few blocks; shapes alone decide. Two
 // blocks run on each of 256 CUs.
 struct Plan {
-  int fwd, per;  // forward: parts over the keys, tiles of each
-  bool few;      // rows fit one wave: attn_rc_few_k, tiles of 32
+  int fwd;       // forward: parts over the keys
+  bool few;      // rows fit one wave: attn_rc_few_k, ...
+  int per;       // ... tiles of 32 in a part
   int dq, dkv;   // backward: parts over the keys, over the rows
   bool whole;    // backward in one pass: attn_rc_bwd_short_k
   bool whole_fwd;  // all keys at once: attn_rc_fwd_short_k
-  // free: no causal mask and no lengths
-  Plan(long b, long sq, long sk, long hk, long g, long hd, bool free) {
+  Plan(long b, long sq, long sk, long hk, long g, long hd, bool causal,
+       bool lens) {
     long bh = b * hk, rows = sq * g;
     // One block a head has to fill the chip, or be short: 4 x 65 tokens of 3
     // heads 10 against 15 us, but 8 x 197 of 12 26 against 24. Sequences of
     // few keys take D from P and dP, which only the two-pass backward does.
-    whole = free && hd <= 64 && sk > 64 && sk <= 256 && rows <= 256 &&
-            (bh >= 256 || (sk <= 128 && rows <= 128));
+    whole = !causal && !lens && hd <= 64 && sk > 64 && sk <= 256 &&
+            rows <= 256 && (bh >= 256 || (sk <= 128 && rows <= 128));
     long rblk = bh * ((rows + 127) / 128), kblk = bh * ((sk + 127) / 128);
     // two of its blocks a CU: 47 against 51 us at 1536 heads of 197 tokens,
     // and no gain below
@@ -1505,6 +1506,16 @@ struct Plan {
     per = 0;
     few = false;
     if (rblk == 0 || kblk == 0) return;
+    // Parts to fill the chip once; twice where there is work enough to pay for
+    // the join of more parts and one round leaves CUs idle or, for a causal
+    // mask, with blocks of different lengths. dQ and its join: 8192 causal
+    // tokens of 4 heads of 64 74 against 99 us, 2048 of 16 heads of 128 63
+    // against 58; 8192 tokens of 6 heads of 64 170 against 193, 4096 of 8 heads
+    // of 128 132 against 118.
+    long want = rblk < 512 ? 512 / rblk : 1;
+    if (rblk < 512 && sk * rblk >= 3 << 19 && (causal || want * rblk < 480))
+      want = 1024 / rblk;
+    int part = clamp(want, sk / 512, 64);
     if (rows <= 32 && sk >= 512) {
       // runs of 256 keys (8 tiles) a wave, longer where that makes more
       // than 4096 waves, 128 where it makes fewer than 1024
@@ -1515,13 +1526,14 @@ struct Plan {
       per = (int)run;
       fwd = (int)((tiles + 2 * run - 1) / (2 * run)) * 2;
     } else {
-      long tiles = (sk + TILE - 1) / TILE;
-      fwd = rblk < 512 ? clamp(1024 / rblk, tiles / 8, 64) : 1;
-      per = (int)((tiles + fwd - 1) / fwd);
+      fwd = part;
     }
-    dq = rblk < 512 ? clamp(1024 / rblk, sk / 512, 64) : 1;
-    // a causal mask's blocks differ in length: more rounds even them out
-    dkv = clamp((1024 + kblk - 1) / kblk, rows / 512, 16);
+    dq = part;
+    // A causal mask's blocks differ in length: where there is work enough to
+    // pay for the join of more parts, two rounds even them out (512 key blocks
+    // of 4096 rows 177 against 195 us, of 2048 rows 119 against 107).
+    bool even = causal && kblk <= 512 && rows >= 4096 && rows * kblk >= 1 << 20;
+    dkv = clamp(((even ? 1024 : 512) + kblk - 1) / kblk, rows / 512, 16);
   }
   static int clamp(long want, long most, long cap) {
     long n = want < most ? want : most;
@@ -1538,8 +1550,8 @@ template <typename T, int HDT>
 void launch(Args a, int bwd, float* ws, hipStream_t s) {
   int rblk = (a.sq * a.g + 127) / 128, kblk = (a.sk + 127) / 128;
   int bh = a.b * a.hk, rblk256 = (a.sq * a.g + 255) / 256;
-  Plan p(a.b, a.sq, a.sk, a.hk, a.g, a.hd,
-         !a.causal && !a.q_lens && !a.kv_lens);
+  Plan p(a.b, a.sq, a.sk, a.hk, a.g, a.hd, a.causal,
+         a.q_lens || a.kv_lens);
   if (!bwd) {
     if (rblk == 0) return;
     if (p.few)
@@ -1549,7 +1561,7 @@ void launch(Args a, int bwd, float* ws, hipStream_t s) {
       attn_rc_fwd_short_k<T><<<bh * rblk256, 512, 0, s>>>(a, rblk256);
     else
       attn_rc_fwd_k<T, HDT>
-          <<<bh * rblk * p.fwd, 256, 0, s>>>(a, rblk, p.fwd, p.per, ws);
+          <<<bh * rblk * p.fwd, 256, 0, s>>>(a, rblk, p.fwd, ws);
     if (p.fwd > 1) {
       long rows = (long)bh * a.sq * a.g;
       if (p.fwd > 8)
@@ -1593,11 +1605,10 @@ void launch(Args a, int bwd, float* ws, hipStream_t s) {
 
 extern "C" {
 
-// floats of workspace that forward or backward needs; free: no causal mask
-// and no lengths
+// floats of workspace that forward or backward needs; lens: there are lengths
 long pdta_attn_recompute_ws(long b, long sq, long sk, long hk, long g,
-                            long hd, int free, int bwd) {
-  Plan p(b, sq, sk, hk, g, hd, free);
+                            long hd, int causal, int lens, int bwd) {
+  Plan p(b, sq, sk, hk, g, hd, causal, lens);
   long nq = b * sq * hk * g * hd, nk = b * sk * hk * hd;
   if (!bwd) return p.fwd > 1 ? p.fwd * (nq + nq / hd) : 0;
   if (p.whole) return 0;

@@ -28,7 +28,8 @@ void pdta_attn_recompute(const void*, const void*, const void*, const void*,
                          const void*, const void*, int, int, int, int,
                          int, int, int, float, int, int, float*, int,
                          hipStream_t);
-long pdta_attn_recompute_ws(long, long, long, long, long, long, int, int);
+long pdta_attn_recompute_ws(long, long, long, long, long, long, int, int,
+                            int);
 }
 
 namespace {
@@ -353,9 +354,9 @@ std::vector<at::Tensor> attn_recompute_fwd(
   attn_strides(k, st + 3);
   attn_strides(v, st + 6);
   if (out.numel()) {
-    bool free = !causal && !q_lens.has_value() && !kv_lens.has_value();
-    long need =
-        pdta_attn_recompute_ws(n.b, n.sq, n.sk, n.hk, g, n.hd, free, 0);
+    bool lens = q_lens.has_value() || kv_lens.has_value();
+    long need = pdta_attn_recompute_ws(n.b, n.sq, n.sk, n.hk, g, n.hd, causal,
+                                       lens, 0);
     at::Tensor ws;
     if (need) ws = at::empty({need}, lse.options());
     pdta_attn_recompute(q.data_ptr(), k.data_ptr(), v.data_ptr(), nullptr,
@@ -401,8 +402,9 @@ std::vector<at::Tensor> attn_recompute_bwd(
                   dv.sizes() == dk.sizes() &&
                   (dv.numel() == 0 || (dv.stride(3) == 1 && rows8(dv))),
               "dv_out must be like v, with aligned rows");
-  bool free = !causal && !q_lens.has_value() && !kv_lens.has_value();
-  long need = pdta_attn_recompute_ws(n.b, n.sq, n.sk, n.hk, g, n.hd, free, 1);
+  bool lens = q_lens.has_value() || kv_lens.has_value();
+  long need = pdta_attn_recompute_ws(n.b, n.sq, n.sk, n.hk, g, n.hd, causal,
+                                     lens, 1);
   at::Tensor ws;
   if (need) ws = at::empty({need}, lse.options());
   long st[15];

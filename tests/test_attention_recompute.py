@@ -543,6 +543,23 @@ def _lengths(n, most):
 
 
 @gpu
+@pytest.mark.parametrize("b,sq,sk,h,hk,hd,causal", [
+    (1, 70, 9000, 1, 1, 64, True),        # keys to many blocks
+    (1, 1300, 1300, 1, 1, 128, True),
+    (1, 1300, 1300, 2, 1, 40, False),
+    (1, 4100, 600, 1, 1, 16, True),       # rows to many; most see nothing
+    (1, 520, 2100, 8, 1, 16, True),
+], ids=str)
+def test_work_dealt_out(b, sq, sk, h, hk, hd, causal):
+    x = _inputs("cuda", torch.float16, b, sq, sk, h, hk, hd)
+    want = _oracle(*x, hd ** -0.5, causal, None, None)
+    got = _run(*x, causal=causal)
+    _check(got, *want)
+    for u, w in zip(got, _run(*x, causal=causal)):
+        assert torch.equal(u, w), "two runs differ"
+
+
+@gpu
 @pytest.mark.parametrize("b,sq,sk,h,hk,hd,ql,kl", [
     (16, 300, 300, 5, 5, 80, True, True),
     (8, 300, 200, 4, 2, 64, True, False),     # lengths of one side
@@ -551,6 +568,7 @@ def _lengths(n, most):
     (66, 140, 140, 4, 4, 72, True, True),     # more: in the batch's order
     (3, 260, 260, 3, 3, 64, True, True),      # heads no multiple of 8
     (4, 130, 1100, 2, 2, 64, True, True),     # keys dealt out and joined
+    (1, 60, 3000, 8, 8, 64, False, True),     # to more than eight
     (8, 1100, 300, 1, 1, 128, True, True),    # rows dealt out and joined
     (8, 40, 1100, 12, 1, 64, True, True),
     (2, 200, 200, 4, 4, 8, True, True),

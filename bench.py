@@ -24,6 +24,7 @@ import torch
 
 from pytorch_distributed_train_amd.flags import build_parser, DistEnv
 from pytorch_distributed_train_amd.engine import Trainer
+from pytorch_distributed_train_amd.parallel.comm import shutdown
 
 
 def parse(argv=None):
@@ -164,6 +165,7 @@ def main(argv=None) -> int:
                 f.write(line + "\n")
         except OSError:
             pass
+    shutdown()
     return 0
 
 

@@ -363,6 +363,16 @@ def _maybe_debug(comm, control):
     return comm
 
 
+def shutdown() -> None:
+    """Ends the process group, when a rank is done. A rank that leaves right
+    behind its last collective can reach the interpreter's end while one of
+    the group's worker threads still lets go of that collective's tensors; a
+    thread that asks for the interpreter then is unwound by force, which
+    ends the process with SIGABRT. Here those threads are joined first."""
+    if torch_dist.is_available() and torch_dist.is_initialized():
+        torch_dist.destroy_process_group()
+
+
 def make_communicator(env: DistEnv, device, backend: str = "auto"):
     """backend: auto|rccl|gloo. auto = rccl on cuda devices, gloo on cpu."""
     if env.world_size <= 1:

@@ -25,6 +25,7 @@ from pytorch_distributed_train_amd.flags import build_parser, DistEnv
 from pytorch_distributed_train_amd.engine import Trainer
 from pytorch_distributed_train_amd.data import (DistributedSampler, Loader,
                                                 make_dataset)
+from pytorch_distributed_train_amd.parallel.comm import shutdown
 from pytorch_distributed_train_amd.utils.checkpoint import (load_checkpoint,
                                                             save_checkpoint)
 from pytorch_distributed_train_amd.utils.metrics import RankLogger, StepTimer
@@ -178,6 +179,7 @@ def main(argv=None):
     if profiler is not None:  # fewer steps ran than --torch-profile
         profiler.__exit__(None, None, None)
     logger.close()
+    shutdown()
     return 0
 
 

@@ -798,7 +798,7 @@ __global__ __launch_bounds__(128, 2) void attn_rc_few_k(Args a, int parts,
 // Groups of 32 lanes, GPR of the block's 8 a row: with many parts a row has
 // all 8, which take the parts in turn, so that all of its loads are out at
 // once; with 8 parts or fewer each group has a row. Parts that saw no key have
-// lse +inf and no output; they come last, as parts take the keys in order.
+// lse +inf and no output; they come last, as parts take the keys in turn.
 template <typename T, int GPR>
 __global__ __launch_bounds__(256) void attn_rc_join_rows_k(Args a, int parts,
                                                            const float* part) {
@@ -830,9 +830,13 @@ __global__ __launch_bounds__(256) void attn_rc_join_rows_k(Args a, int parts,
   int at = d < a.hd ? d : 0;  // lanes past the head load and drop its start
 #pragma unroll 4
   for (int p = grp; p < used; p += GPR) {
-    float w = __builtin_amdgcn_exp2f(ls[p * rows] - top);
     float4 x =
         *reinterpret_cast<const float4*>(part + (p * rows + r) * a.hd + at);
+    // a part whose scores are all -inf has no output either
+    bool none = ls[p * rows] == INFINITY;
+    float w = none ? 0.f : __builtin_amdgcn_exp2f(ls[p * rows] - top);
+    x.x = none ? 0.f : x.x, x.y = none ? 0.f : x.y;
+    x.z = none ? 0.f : x.z, x.w = none ? 0.f : x.w;
     sum += w;
     acc.x += w * x.x, acc.y += w * x.y, acc.z += w * x.z, acc.w += w * x.w;
   }

@@ -587,3 +587,24 @@ def test_lengths_in_any_order(b, sq, sk, h, hk, hd, ql, kl):
     del stale
     got = _run(q, k, v, do, q_lens=_t(ql, "cuda"), kv_lens=_t(kl, "cuda"))
     _check(got, *want)
+
+
+@gpu
+@pytest.mark.parametrize("sq", [1, 70])  # a wave's runs; tiles in turn
+def test_scores_of_minus_infinity(sq):
+    """Products past fp32's range make the first 640 keys' scores -inf, which
+    empties the first parts of what is dealt out; the others' are 0, so an
+    output is their mean, rounded once (and P once more)."""
+    q, k, v, do = _inputs("cuda", torch.bfloat16, 1, sq, 1500, 1, 1, 64)
+    q.fill_(2.0 ** 70)
+    k.zero_()
+    k[:, :640] = -2.0 ** 70
+    # NaN where an unwritten part would be read
+    stale = torch.full((1 << 22,), float("nan"), device="cuda")
+    del stale
+    got = _run(q, k, v, do)
+    want = v[:, 640:].double().mean(1, keepdim=True)
+    tol = 2 * 2.0 ** -8 * v[:, 640:].double().abs().mean(1, keepdim=True)
+    assert bool(((got[0].double() - want).abs() <= tol).all())
+    assert all(bool(x.isfinite().all()) for x in got[:2])
+    assert not bool(got[2][:, :640].any()) and not bool(got[3][:, :640].any())

@@ -164,8 +164,8 @@ DEV_INLINE int wave_scan(int x) {
 // to one CU after the other, two each; so a head's blocks stay on a die, and
 // the first 32 go there from short to long, so that the long ones share their
 // CU with the shortest of the next 32. 16 sequences of 0 to 777 tokens, 10
-// heads of 80: forward 34 us, dQ 43, dK/dV 53; in the order of the batch 40,
-// 49, 66. A block spends 1.4 us here; the longest run 20.
+// heads of 80: forward 34 us, dQ 41, dK/dV 51; in the order of the batch each
+// took 6 to 13 us more. A block spends 1.4 us here, the longest 21 on its run.
 // Lane l ranks sequence l (b <= 64) and then places head die + 8 l; heads are
 // a multiple of 8 up to 512.
 template <bool KEYS, int BLOCK>
